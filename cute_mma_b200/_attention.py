@@ -1,0 +1,218 @@
+"""Attention of the decoder that Prism layers stand in: whole prompts (``causal_attention``, differentiable) and single
+tokens (``decode_attention``).
+
+The reference's training model calls PyTorch's attention between its Prism layers (integration/model.py:95-117); here
+it is the library's own kernels, so that queries, keys and values are read where the QKV layer's output holds them
+(column ranges of one matrix) and sequences of different lengths are packed without padding.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _functional as F
+from . import _lib
+from ._module import _plain_eager, _plain_grad
+
+_STRIDES9, _STRIDES12 = ctypes.c_longlong * 9, ctypes.c_longlong * 12
+
+
+def _check_heads(q, k, v) -> None:
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor, got device={t.device}")
+        if t.dtype not in F._DTYPES:
+            raise ValueError(f"{name} must be float16 or bfloat16, got dtype={t.dtype}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"All tensors must have the same dtype, got q={q.dtype}, k={k.dtype}, v={v.dtype}")
+    if not (q.device == k.device == v.device):
+        raise ValueError("All tensors must be on the same CUDA device")
+    if k.shape != v.shape:
+        raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"head_dim mismatch: q has {q.shape[-1]} but k has {k.shape[-1]}")
+    d, hq, hkv = q.shape[-1], q.shape[-2], k.shape[-2]
+    if d % 8 != 0 or not 8 <= d <= 128:
+        raise ValueError(f"head_dim must be a multiple of 8 up to 128 for the sm_100a kernels, got {d}")
+    if hkv < 1 or hq < 1 or hq % hkv != 0:
+        raise ValueError(f"the heads of q ({hq}) must be a multiple of those of k and v ({hkv})")
+
+
+def _check_scale(scale, head_dim) -> float:
+    if scale is None:
+        return head_dim ** -0.5
+    scale = float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
+
+
+def _check_prompt(q, k, v, cu_seqlens) -> None:
+    if not (q.dim() == k.dim() == v.dim()) or q.dim() not in (3, 4):
+        raise ValueError("q, k and v must be 3D (rows, heads, head_dim) or 4D (batch, rows, heads, head_dim), "
+                         f"got {q.dim()}D, {k.dim()}D and {v.dim()}D")
+    _check_heads(q, k, v)
+    if q.shape[:-2] != k.shape[:-2]:
+        raise ValueError(f"q and k must have the same rows, got {tuple(q.shape[:-2])} and {tuple(k.shape[:-2])}")
+    if q.shape[:-2].numel() >= 1 << 31:
+        raise ValueError("more than 2^31 rows")
+    if cu_seqlens is None:
+        return
+    if q.dim() != 3:
+        raise ValueError("cu_seqlens goes with packed (rows, heads, head_dim) tensors")
+    if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2
+            or not cu_seqlens.is_contiguous() or cu_seqlens.device != q.device):
+        raise ValueError("cu_seqlens must be a contiguous int32 tensor (sequences + 1,) on the device of q")
+
+
+def _tma_rows(t):
+    """t as the kernels can read it: features contiguous, 16-byte steps between rows, heads and batches (a copy where
+    that is not so, e.g. of an expanded tensor), and its (batch, row, head) strides."""
+    d = t.shape[-1]
+
+    def steps(x):
+        s = [8 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride()[:-1])]   # a single entry has no stride
+        return s if len(s) == 3 else [8] + s
+
+    s = steps(t)
+    if t.stride(-1) != 1 or any(x <= 0 or x % 8 for x in s) or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        s = steps(t)
+    return t, s
+
+
+def _attn_forward(q, k, v, cu_seqlens, scale, want_lse):
+    """(o, lse or None); q, k, v as checked."""
+    hq, d = q.shape[-2:]
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rows = q.shape[:-2].numel()
+    lse = torch.empty(hq, rows, dtype=torch.float32, device=q.device) if want_lse else None
+    if rows == 0:
+        return o, lse
+    q, sq = _tma_rows(q)
+    k, sk = _tma_rows(k)
+    v, sv = _tma_rows(v)
+    n, length = _sequences(q, cu_seqlens)
+    with F._device_scope(q.device):
+        ws = F._workspace.get(q.device, 256)
+        _lib.check(_lib.lib().prism_attn_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), F._ptr(lse), F._ptr(cu_seqlens), n, length, rows,
+            hq, k.shape[-2], d, F._DTYPES[q.dtype], scale, _STRIDES9(*sq, *sk, *sv), ws.data_ptr(), ws.numel(),
+            F._raw_stream(q.device)))
+    return o, lse
+
+
+def _sequences(q, cu_seqlens):
+    """(number of sequences, rows of each; rows 0 where cu_seqlens holds them)."""
+    if cu_seqlens is not None:
+        return cu_seqlens.numel() - 1, 0
+    return (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+
+
+def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_dkv=True):
+    """(dq, dk, dv), None for what is not asked for."""
+    hq, d = q.shape[-2:]
+    rows = q.shape[:-2].numel()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_dq else None
+    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if need_dkv else None for _ in range(2))
+    if rows == 0 or not (need_dq or need_dkv):
+        return dq, dk, dv
+    o = o.contiguous()
+    d_o, sdo = _tma_rows(d_o)
+    q, sq = _tma_rows(q)
+    k, sk = _tma_rows(k)
+    v, sv = _tma_rows(v)
+    n, length = _sequences(q, cu_seqlens)
+    with F._device_scope(q.device):
+        delta = torch.empty(hq, rows, dtype=torch.float32, device=q.device)
+        ws = F._workspace.get(q.device, 256)
+        _lib.check(_lib.lib().prism_attn_bwd(
+            d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), F._ptr(dq), F._ptr(dk),
+            F._ptr(dv), delta.data_ptr(), F._ptr(cu_seqlens), n, length, rows, hq, k.shape[-2], d, F._DTYPES[q.dtype],
+            scale, _STRIDES12(*sq, *sk, *sv, *sdo), ws.data_ptr(), ws.numel(), F._raw_stream(q.device)))
+    return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------
+# custom ops (traced, compiled and transformed calls) and the eager autograd node, as for the layer itself
+# ---------------------------------------------------------------------------
+@torch.library.custom_op("prism_b200::causal_attention", mutates_args=())
+def _attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None,
+                  scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return _attn_forward(q, k, v, cu_seqlens, scale, True)
+
+
+@_attention_op.register_fake
+def _(q, k, v, cu_seqlens, scale):
+    return q.new_empty(q.shape), q.new_empty((q.shape[-2], q.shape[:-2].numel()), dtype=torch.float32)
+
+
+@torch.library.custom_op("prism_b200::causal_attention_backward", mutates_args=())
+def _attention_bwd_op(d_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                      lse: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale)
+
+
+@_attention_bwd_op.register_fake
+def _(d_o, q, k, v, o, lse, cu_seqlens, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+def _attention_setup(ctx, inputs, output):
+    q, k, v, cu_seqlens, scale = inputs
+    ctx.save_for_backward(q, k, v, *output, cu_seqlens)
+    ctx.scale = scale
+    ctx.mark_non_differentiable(output[1])
+
+
+def _attention_grad(ctx, d_o, _d_lse):
+    q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+    return *_attention_bwd_op(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale), None, None
+
+
+_attention_op.register_autograd(_attention_grad, setup_context=_attention_setup)
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, scale):
+        o, lse = _attn_forward(q, k, v, cu_seqlens, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o):
+        q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+        if _plain_eager(d_o, q, k, v, o, lse) and _plain_grad(d_o):
+            need = ctx.needs_input_grad
+            dq, dk, dv = _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale, need[0], need[1] or need[2])
+            return dq, dk if need[1] else None, dv if need[2] else None, None, None
+        return *_attention_bwd_op(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale), None, None
+
+
+def causal_attention(q, k, v, cu_seqlens=None, scale=None):
+    """``softmax(scale * q @ k^T, keys up to the query's own row) @ v`` for every head of every sequence; differentiable.
+
+    Packed: q ``(rows, heads, head_dim)``, k and v ``(rows, kv_heads, head_dim)`` with ``cu_seqlens``
+    ``(sequences + 1,)`` int32 on the same device, sequence i in rows ``cu_seqlens[i]`` up to ``cu_seqlens[i + 1]``
+    (ascending; lengths of zero are allowed; never read by the host).  Rows that belong to no sequence are zeros in the
+    output and in the gradients.  Without ``cu_seqlens`` the tensors are one sequence, or, 4D
+    ``(batch, rows, heads, head_dim)``, a batch of them.  float16 or bfloat16; ``heads`` a multiple of ``kv_heads``
+    (neighbouring query heads share a key head); ``head_dim`` a multiple of 8 up to 128; ``scale`` positive, by default
+    ``head_dim ** -0.5``.  Column ranges of one QKV matrix are read in place.
+    Probabilities are rounded to the inputs' type before they meet ``v``, everything else is summed in fp32.
+    """
+    _check_prompt(q, k, v, cu_seqlens)
+    scale = _check_scale(scale, q.shape[-1])
+    if _plain_eager(q, k, v, cu_seqlens):
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _AttentionFn.apply(q, k, v, cu_seqlens, scale)
+        return _attn_forward(q, k, v, cu_seqlens, scale, False)[0]
+    return _attention_op(q, k, v, cu_seqlens, scale)[0]

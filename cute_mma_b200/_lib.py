@@ -16,8 +16,9 @@ _CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.environ.get("PRISM_B200_LIB", os.path.join(_HERE, "libprism_b200.so"))
 SOURCES = ["prism_abi.cu", "prism_fwd.cu", "prism_fwd_small.cu", "prism_bwd_db.cu", "prism_bwd_dadr.cu",
            "prism_bwd_dadr_f16.cu", "prism_bwd_dadr_bf16.cu", "prism_fwd_noalloc.cu", "prism_cayley.cu", "prism_peer_reduce.cu",
-           "prism_shuffle.cu"]
-HEADERS = ["prism_common.cuh", "prism_host.cuh", "prism_kernels.cuh", "prism_bwd_dadr_kernel.cuh", "prism_plan.h"]
+           "prism_shuffle.cu", "prism_decoder_abi.cu", "prism_attn_fwd.cu", "prism_attn_bwd.cu"]
+HEADERS = ["prism_common.cuh", "prism_host.cuh", "prism_kernels.cuh", "prism_bwd_dadr_kernel.cuh", "prism_plan.h", "prism_attn.cuh",
+           "prism_attn_host.cuh"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(_HERE), "include", "prism_b200.h")
 
 NVCC_FLAGS = [
@@ -29,7 +30,7 @@ NVCC_FLAGS = [
 EXPORTS = [
     "prism_fwd", "prism_fwd_dropout", "prism_fwd_noalloc", "prism_bwd_dadr", "prism_bwd_db", "prism_dbias", "prism_fold_weight", "prism_cayley", "prism_cayley_bwd", "prism_peer_reduce",
     "prism_bwd_dadr_mask", "prism_bwd_db_mask", "prism_dropout_mask_bytes", "prism_shuffle_cols", "prism_shuffle_fold_r", "prism_shuffle_unfold_r", "prism_workspace_bytes",
-    "prism_status",
+    "prism_status", "prism_attn_fwd", "prism_attn_bwd",
     "prism_last_error_string", "prism_abi_version", "prism_launch_count",
 ]
 
@@ -153,6 +154,14 @@ def lib() -> ctypes.CDLL:
             L.prism_shuffle_unfold_r.argtypes = [vp, vp, vp, i, i, i, vp]
             L.prism_peer_reduce.restype = i
             L.prism_peer_reduce.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(vp), i, i, ll, i, ctypes.c_float, i, vp]
+            missing = [name for name in EXPORTS if not hasattr(L, name)]
+            if missing:
+                raise RuntimeError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it (cute_mma_b200._lib.build(force=True))")
+            llp, fl = ctypes.POINTER(ll), ctypes.c_float
+            L.prism_attn_fwd.restype = i
+            L.prism_attn_fwd.argtypes = [vp] * 6 + [i] * 7 + [fl, llp, vp, sz, vp]
+            L.prism_attn_bwd.restype = i
+            L.prism_attn_bwd.argtypes = [vp] * 11 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_workspace_bytes.restype = sz
             L.prism_workspace_bytes.argtypes = [i, i, i, i, i, i, i, ip]
             L.prism_status.restype = i

@@ -206,6 +206,25 @@ int prism_shuffle_unfold_r(const void* dR64, void* dR, const unsigned char* seg,
 int prism_peer_reduce(const void* const* in_ptrs, void* const* out_ptrs, int world, int rank, long long n,
                       int out_dtype, float scale, int ctas, void* stream);
 
+/* Causal attention over whole prompts, of the decoder that the layers stand in (the reference calls PyTorch's,
+ * integration/model.py:95-117): o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j for every head of every sequence.
+ * q: rows x heads x head_dim, k and v: rows x kv_heads x head_dim (heads a multiple of kv_heads: heads h * heads / kv_heads
+ * and on share k and v of head h), features contiguous, head_dim a multiple of 8 up to 128.
+ * cu_seqlens (device, n_seqs + 1 int32, or NULL): row ranges of packed sequences; offsets are taken into [0, rows] and
+ * never backwards, and rows that belong to no sequence are zeros in every output.  NULL: n_seqs sequences of seq_len rows
+ * (rows = n_seqs * seq_len).  strides (host): {batch, row, head} in elements for q, k, v (batch: dense only), multiples of
+ * 8; pointers 16-byte aligned.  o: contiguous.  lse: NULL, or heads x rows fp32 for prism_attn_bwd.  The scale is positive.
+ * Backward: d_o with strides[9..11], o and lse of the forward; dq, dk, dv contiguous, dq or both of dk and dv NULL where they are
+ * not wanted; delta: scratch, heads x rows fp32.  All sums have one owner: bit-stable.
+ * workspace: its status header (PRISM_WORKSPACE_HEADER_BYTES). */
+int prism_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu_seqlens, int n_seqs,
+                   int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+                   const long long* strides, void* workspace, size_t workspace_bytes, void* stream);
+int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                   void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len, int rows,
+                   int heads, int kv_heads, int head_dim, int dtype, float scale, const long long* strides,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Bytes of workspace the given call needs (kind = PRISM_KIND_*), header included. */
 size_t prism_workspace_bytes(int kind, int M, int N, int K, int group_size, int reconn_sz,
                              int dtype, const int* cfg);
