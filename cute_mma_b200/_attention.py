@@ -16,7 +16,7 @@ from . import _functional as F
 from . import _lib
 from ._module import _plain_eager, _plain_grad
 
-_STRIDES9, _STRIDES12 = ctypes.c_longlong * 9, ctypes.c_longlong * 12
+_STRIDES8, _STRIDES9, _STRIDES12 = (ctypes.c_longlong * n for n in (8, 9, 12))
 
 
 def _check_heads(q, k, v) -> None:
@@ -216,3 +216,70 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
             return _AttentionFn.apply(q, k, v, cu_seqlens, scale)
         return _attn_forward(q, k, v, cu_seqlens, scale, False)[0]
     return _attention_op(q, k, v, cu_seqlens, scale)[0]
+
+
+# ---------------------------------------------------------------------------
+# single tokens
+# ---------------------------------------------------------------------------
+def _check_decode(q, k, v, lengths) -> None:
+    if q.dim() != 3 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q must be 3D (sequences, heads, head_dim), k and v 4D (sequences, room, kv_heads, head_dim), "
+                         f"got {q.dim()}D, {k.dim()}D and {v.dim()}D")
+    _check_heads(q, k, v)
+    if q.shape[0] != k.shape[0]:
+        raise ValueError(f"q and k must have the same sequences, got {q.shape[0]} and {k.shape[0]}")
+    if k.shape[1] >= 1 << 31 or q.shape[0] * q.shape[1] >= 1 << 31:
+        raise ValueError("more than 2^31 rows")
+    if (lengths.dtype != torch.int32 or lengths.shape != (q.shape[0],) or not lengths.is_contiguous()
+            or lengths.device != q.device):
+        raise ValueError("lengths must be a contiguous int32 tensor (sequences,) on the device of q")
+    for name, t in (("k", k), ("v", v)):
+        # (a copy of a whole cache per token is not what a caller wants)
+        if t.numel() and (t.stride(-1) != 1 or any(s % 8 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
+                          or t.data_ptr() % 16):
+            raise ValueError(f"{name} must have contiguous features, strides that are multiples of 8 elements and start "
+                             "on a 16-byte boundary")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError("decode_attention has no backward pass; call it under torch.no_grad(), or causal_attention")
+
+
+@torch.library.custom_op("prism_b200::decode_attention", mutates_args=())
+def _decode_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, scale: float) -> torch.Tensor:
+    return _decode(q, k, v, lengths, scale)
+
+
+@_decode_op.register_fake
+def _(q, k, v, lengths, scale):
+    return q.new_empty(q.shape)
+
+
+def _decode(q, k, v, lengths, scale):
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    b, hq, d = q.shape
+    if b == 0:
+        return o
+    q, sq = _tma_rows(q)
+    steps = [[0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])] for t in (k, v)]
+    L = _lib.lib()
+    with F._device_scope(q.device):
+        nbytes = L.prism_attn_decode_scratch_bytes(d)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _lib.check(L.prism_attn_decode(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lengths.data_ptr(), b, k.shape[1], hq, k.shape[2], d,
+            F._DTYPES[q.dtype], scale, _STRIDES8(sq[1], sq[2], *steps[0], *steps[1]), scratch.data_ptr(), nbytes,
+            F._raw_stream(q.device)))
+    return o
+
+
+def decode_attention(q, k, v, lengths, scale=None):
+    """Attention of the newest token of every sequence over that sequence's keys and values, without gradients.
+
+    q ``(sequences, heads, head_dim)``; k, v ``(sequences, room, kv_heads, head_dim)`` of any strides with contiguous
+    features and 16-byte steps (a slice of a larger cache is read in place); ``lengths`` ``(sequences,)`` int32 on the
+    same device: the rows of k and v that count, the newest token's own among them; nothing behind them is read, so
+    that it may hold anything.  A length of 0 gives a row of zeros; lengths are taken into ``[0, room]`` and never read by
+    the host.  Types, heads and ``scale`` as for ``causal_attention``.
+    """
+    _check_decode(q, k, v, lengths)
+    scale = _check_scale(scale, q.shape[-1])
+    return (_decode if _plain_eager(q, k, v, lengths) else _decode_op)(q, k, v, lengths, scale)

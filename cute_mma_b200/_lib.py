@@ -16,9 +16,10 @@ _CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.environ.get("PRISM_B200_LIB", os.path.join(_HERE, "libprism_b200.so"))
 SOURCES = ["prism_abi.cu", "prism_fwd.cu", "prism_fwd_small.cu", "prism_bwd_db.cu", "prism_bwd_dadr.cu",
            "prism_bwd_dadr_f16.cu", "prism_bwd_dadr_bf16.cu", "prism_fwd_noalloc.cu", "prism_cayley.cu", "prism_peer_reduce.cu",
-           "prism_shuffle.cu", "prism_decoder_abi.cu", "prism_attn_fwd.cu", "prism_attn_bwd.cu"]
+           "prism_shuffle.cu", "prism_decoder_abi.cu", "prism_attn_fwd.cu", "prism_attn_bwd.cu",
+           "prism_attn_decode.cu", "prism_norm.cu"]
 HEADERS = ["prism_common.cuh", "prism_host.cuh", "prism_kernels.cuh", "prism_bwd_dadr_kernel.cuh", "prism_plan.h", "prism_attn.cuh",
-           "prism_attn_host.cuh"]
+           "prism_attn_host.cuh", "prism_norm.cuh"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(_HERE), "include", "prism_b200.h")
 
 NVCC_FLAGS = [
@@ -30,7 +31,8 @@ NVCC_FLAGS = [
 EXPORTS = [
     "prism_fwd", "prism_fwd_dropout", "prism_fwd_noalloc", "prism_bwd_dadr", "prism_bwd_db", "prism_dbias", "prism_fold_weight", "prism_cayley", "prism_cayley_bwd", "prism_peer_reduce",
     "prism_bwd_dadr_mask", "prism_bwd_db_mask", "prism_dropout_mask_bytes", "prism_shuffle_cols", "prism_shuffle_fold_r", "prism_shuffle_unfold_r", "prism_workspace_bytes",
-    "prism_status", "prism_attn_fwd", "prism_attn_bwd",
+    "prism_status", "prism_attn_fwd", "prism_attn_bwd", "prism_attn_decode", "prism_attn_decode_scratch_bytes",
+    "prism_layer_norm", "prism_layer_norm_bwd", "prism_layer_norm_scratch_bytes",
     "prism_last_error_string", "prism_abi_version", "prism_launch_count",
 ]
 
@@ -162,6 +164,16 @@ def lib() -> ctypes.CDLL:
             L.prism_attn_fwd.argtypes = [vp] * 6 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_attn_bwd.restype = i
             L.prism_attn_bwd.argtypes = [vp] * 11 + [i] * 7 + [fl, llp, vp, sz, vp]
+            L.prism_attn_decode_scratch_bytes.restype = sz
+            L.prism_attn_decode_scratch_bytes.argtypes = [i]
+            L.prism_attn_decode.restype = i
+            L.prism_attn_decode.argtypes = [vp] * 5 + [i] * 6 + [fl, llp, vp, sz, vp]
+            L.prism_layer_norm.restype = i
+            L.prism_layer_norm.argtypes = [vp] * 8 + [ll, i, i, i, fl, ll, ll, vp]
+            L.prism_layer_norm_scratch_bytes.restype = sz
+            L.prism_layer_norm_scratch_bytes.argtypes = [ll, i]
+            L.prism_layer_norm_bwd.restype = i
+            L.prism_layer_norm_bwd.argtypes = [vp] * 9 + [ll, i, i, i, ll, ll, ll, vp, sz, vp]
             L.prism_workspace_bytes.restype = sz
             L.prism_workspace_bytes.argtypes = [i, i, i, i, i, i, i, ip]
             L.prism_status.restype = i

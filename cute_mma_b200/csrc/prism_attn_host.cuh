@@ -29,6 +29,9 @@ struct AttnArgs {
 
 int launch_attn_fwd(const AttnArgs& a);
 int launch_attn_bwd(const AttnArgs& a);
+// q: n rows (strides batch and head), k and v: n x len rows, lengths [n]; scratch: attn_decode_scratch_bytes.
+int launch_attn_decode(const AttnArgs& a, const int* lengths, float* scratch, int num_sms);
+size_t attn_decode_scratch_bytes(int dim, int num_sms);
 
 // Tiles of bm rows over all sequences.  Packed: the lengths stand on the GPU; n sequences of `rows` rows have at most
 // (rows + n (bm - 1)) / bm tiles, and one more CTA row sees to the rows of no sequence.

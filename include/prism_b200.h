@@ -225,6 +225,32 @@ int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v,
                    int heads, int kv_heads, int head_dim, int dtype, float scale, const long long* strides,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of one query row per sequence over its keys and values so far (serving: the next token).
+ * q, o: n_seqs x heads x head_dim; k, v: n_seqs x room x kv_heads x head_dim, of which the first lengths[i] rows of sequence
+ * i count (device int32, taken into [0, room]; 0: a row of zeros) and only they are read.  strides (host): q {batch, head},
+ * k {batch, row, head}, v {batch, row, head}, in elements, multiples of 8 (0 allowed); 16-byte aligned pointers; o contiguous.
+ * scratch: prism_attn_decode_scratch_bytes bytes, 16-byte aligned, any contents, not shared by calls that overlap. */
+size_t prism_attn_decode_scratch_bytes(int head_dim);
+int prism_attn_decode(const void* q, const void* k, const void* v, void* o, const int* lengths, int n_seqs, int room,
+                      int heads, int kv_heads, int head_dim, int dtype, float scale, const long long* strides,
+                      void* scratch, size_t scratch_bytes, void* stream);
+
+/* Layer norm of rows x cols 16-bit values, as it stands before the decoder's linears: s = x (+ residual, rounded to the
+ * rows' type and written to sum), y = (s - mean) / sqrt(variance + eps) * weight + bias; statistics in fp32, of deviations
+ * from the mean.  weight, bias [cols]: fp32 or of the rows' type (w_dtype); bias may be NULL.  ldx, ldr: row strides of x
+ * and residual in elements (any); y and sum contiguous.  mean, rstd: NULL, or [rows] fp32 for the backward.  cols up to
+ * 16384.  Backward: s is what was normalised (x or sum); dx = gradient through y, plus dsum where given (NULL: none);
+ * dweight, dbias as weight, NULL where not wanted; their sums over the rows are added in a fixed order (bit-stable) through scratch
+ * (prism_layer_norm_scratch_bytes bytes, any contents, not shared by calls that overlap). */
+int prism_layer_norm(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* sum,
+                     float* mean, float* rstd, long long rows, int cols, int dtype, int w_dtype, float eps, long long ldx,
+                     long long ldr, void* stream);
+size_t prism_layer_norm_scratch_bytes(long long rows, int cols);
+int prism_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const void* weight, const float* mean,
+                         const float* rstd, void* dx, void* dweight, void* dbias, long long rows, int cols, int dtype,
+                         int w_dtype, long long lddy, long long ldds, long long lds, void* scratch, size_t scratch_bytes,
+                         void* stream);
+
 /* Bytes of workspace the given call needs (kind = PRISM_KIND_*), header included. */
 size_t prism_workspace_bytes(int kind, int M, int N, int K, int group_size, int reconn_sz,
                              int dtype, const int* cfg);
