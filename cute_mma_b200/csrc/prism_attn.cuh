@@ -86,14 +86,14 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, int idx, int bm
   return w;
 }
 
-// Rows of a packed batch that belong to no sequence, [0, cu[0]) and [cu[n], rows), are zeros in every output: written by
-// the CTAs that got no tile.  out: rows x heads x dim, this CTA's head; 16-byte pieces.
+// Rows of a packed batch that belong to no sequence, [0, cu[0]) and [cu[n], rows), are zeros in every output: written for
+// the tiles of the grid that there are none of.  out: rows x heads x dim; one warp, one head, 16-byte pieces.
 __device__ __forceinline__ void attn_zero_gap(const AttnRows& r, const AttnWork& w, uint16_t* out, int heads, int head,
                                               int dim) {
-  const int front = attn_clamp(__ldg(r.cu), 0, r.rows), end = attn_clamp(__ldg(r.cu + r.n), 0, r.rows);
-  const int pieces = dim >> 3;
+  const int front = attn_clamp(__ldg(r.cu), 0, r.rows), end = attn_clamp(__ldg(r.cu + r.n), front, r.rows);
+  const int pieces = dim >> 3, lane = threadIdx.x & 31;
   const long long gap = (long long)front + (r.rows - end);
-  for (long long i = (long long)w.spare * blockDim.x + threadIdx.x; i < gap * pieces; i += (long long)w.n_spare * blockDim.x) {
+  for (long long i = (long long)w.spare * 32 + lane; i < gap * pieces; i += (long long)w.n_spare * 32) {
     const long long g = i / pieces;
     const long long row = g < front ? g : end + (g - front);
     reinterpret_cast<uint4*>(out + (row * heads + head) * dim)[i - g * pieces] = make_uint4(0u, 0u, 0u, 0u);
@@ -103,6 +103,136 @@ __device__ __forceinline__ void attn_zero_gap(const AttnRows& r, const AttnWork&
 // A bounded wait by a whole warp, which stays together: false for all lanes if it ran out for one.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// The work of a CTA: it begins with the tile of its own block index and then takes over blocks that have not started yet
+// (cluster launch control), so that the loads and first products of the next tile run beside the end of this one and no
+// CTA is set up twice.  One warp of the CTA looks for work ahead and hands it to the others through two slots.
+struct AttnSched {
+  uint64_t full[2], empty[2], answer_full;
+  alignas(16) uint64_t answer[2];
+  AttnWork work[2];
+  int head[2];
+};
+__device__ __forceinline__ void attn_sched_init(AttnSched& s, uint32_t consumers) {
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&s.full[i], 1);
+    mbar_init(&s.empty[i], consumers);
+  }
+  mbar_init(&s.answer_full, 1);
+}
+__device__ __forceinline__ void clc_try_cancel(uint64_t* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               :
+               : "r"(smem_u32(answer)), "r"(smem_u32(bar))
+               : "memory");
+}
+// The x index of the block taken over, or -1 where there is none left.
+__device__ __forceinline__ int clc_answer(const uint64_t* answer) {
+  uint32_t took, x;
+  asm volatile(
+      "{\n\t"
+      ".reg .b128 h;\n\t"
+      ".reg .pred p;\n\t"
+      "mov.b128 h, {%2, %3};\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "mov.b32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t"
+      "}\n"
+      : "=r"(took), "=r"(x)
+      : "l"(answer[0]), "l"(answer[1]));
+  return took ? (int)x : -1;
+}
+
+// The warp that looks for work.  zero(work, head): what to do for a tile that there is none of.
+template <typename Zero>
+__device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows, int heads, int bm, bool last_first, Zero zero) {
+  const int lane = threadIdx.x & 31;
+  Ring r(2);
+  uint32_t phase = 0;
+  int idx = blockIdx.x;
+  while (idx >= 0) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&s.answer_full, 16);
+      clc_try_cancel(s.answer, &s.answer_full);
+    }
+    const int head = idx % heads;
+    const AttnWork w = attn_find(rows, idx / heads, bm, last_first);
+    if (w.tile < 0) {
+      zero(w, head);
+    } else {
+      if (!warp_wait(&s.empty[r.idx], r.phase ^ 1)) {
+        warp_wait(&s.answer_full, phase);   // its answer is still on the way into this CTA's memory
+        return false;
+      }
+      if (lane == 0) {
+        s.work[r.idx] = w;
+        s.head[r.idx] = head;
+        mbar_arrive(&s.full[r.idx]);
+      }
+      r.next();
+    }
+    if (!warp_wait(&s.answer_full, phase)) return false;
+    phase ^= 1u;
+    idx = clc_answer(s.answer);
+    fence_proxy_async_smem();   // the answer is read before the next one may overwrite it
+    __syncwarp();
+  }
+  if (!warp_wait(&s.empty[r.idx], r.phase ^ 1)) return false;
+  if (lane == 0) {
+    s.work[r.idx].tile = -1;
+    mbar_arrive(&s.full[r.idx]);
+  }
+  return true;
+}
+// The next piece of work for one of the other warps: false at the end (or if the wait ran out, with ok false).
+__device__ __forceinline__ bool attn_next(AttnSched& s, Ring& r, AttnWork* w, int* head, bool* ok) {
+  if (!warp_wait(&s.full[r.idx], r.phase)) { *ok = false; return false; }
+  *w = s.work[r.idx];
+  *head = s.head[r.idx];
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&s.empty[r.idx]);
+  r.next();
+  return w->tile >= 0;
+}
+
+// 2^x for two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], a polynomial of degree 5 for 2^f (least largest
+// relative error with the constant fixed to 1, by linear programming: 1.9e-7 in fp32) times 2^n.  Below 2^-126 the result
+// stays at 2^-126 (of a largest probability of 1); NaN stays NaN.  The special function unit makes 16 of these a clock and
+// SM, a quarter of what one tile of 128 x 128 scores per 1024 clocks of products needs together with the rest: part of
+// the exponentials are done here.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t"
+      "}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 ex2_poly2(float2 x) {
+  x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
+  const float2 t = add2(x, both(12582912.f));                       // n in the low bits
+  const float2 f = add2(x, mul2(add2(t, both(-12582912.f)), both(-1.f)));
+  float2 p = fma2(f, both(0x1.5bb994p-10f), both(0x1.3cea84p-7f));
+  p = fma2(p, f, both(0x1.c6b754p-5f));
+  p = fma2(p, f, both(0x1.ebf9bcp-3f));
+  p = fma2(p, f, both(0x1.62e42ap-1f));
+  p = fma2(p, f, both(1.f));
+  const float2 s = make_float2(__uint_as_float(__float_as_uint(t.x) * 0x800000u + 0x3f800000u),
+                               __uint_as_float(__float_as_uint(t.y) * 0x800000u + 0x3f800000u));
+  return mul2(p, s);
 }
 
 // 2^x, the hardware's approximation (2 ulp); -infinity gives 0.
@@ -116,7 +246,7 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) { return max_nan(max_nan(a, b), c); }
 
 // Registers -> TMEM: 32 consecutive columns of the thread's own lane.
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
@@ -129,6 +259,16 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 

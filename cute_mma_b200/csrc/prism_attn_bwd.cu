@@ -21,7 +21,14 @@ struct BwdParams {
   int* err;
 };
 
-constexpr int kThreads = 384;   // two warpgroups of arithmetic, MMA warp, TMA warp, warp of the row statistics
+// Two warpgroups of arithmetic, then the MMA warp, the TMA warp, the warp of the row statistics and the one that looks for
+// work.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is launched with.
+constexpr int kThreads = 384, kMathRegs = 208, kOtherRegs = 88;
+
+// Every PRISM_ATTN_BWD_POLY-th second pair of exponentials goes to the FMA pipe.
+#ifndef PRISM_ATTN_BWD_POLY
+#define PRISM_ATTN_BWD_POLY 2
+#endif
 
 // ---------------------------------------------------------------------------------------------------- delta
 // Sixteen lanes a row of a head: 16-byte pieces of o and do.
@@ -60,15 +67,18 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const DeltaParams p) {
 // Transposed scores: S^T = K Q^T and dP^T = V dO^T have a key row per TMEM lane, so that P^T and dS^T, written back over
 // them in 16 bits, are the TMEM operands of dv += P^T dO and dk += dS^T Q.  The row statistics lie along the columns and
 // are read from shared memory, the same word by all lanes.  Rows behind the sequence get lse = +infinity: P = 0.
+// Each warpgroup has 64 of the 128 query columns.  P goes over in two pieces of 32 columns of each, so that dv's product
+// starts in the middle of the exponentials.  Heads of up to 64 leave TMEM for a second S buffer: the next scores are then
+// formed beside this tile's exponentials; wider heads form them behind dv's product, which frees S.
 template <int DH>
 struct DkvSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
-  static constexpr int kRing = 2;   // pairs of Q and dO tiles
-  static constexpr uint32_t kBytes = (2 + 2 * kRing) * kTile + 1024;
+  static constexpr int kQ = DH == 128 ? 3 : 4, kDo = DH == 128 ? 2 : 4;   // rings of Q and of dO tiles
+  static constexpr uint32_t kBytes = (2 + kQ + kDo) * kTile + 1024;
 };
 struct DkvBars {
-  uint64_t kv_full, s_full, p_full, dp_full, ds_full, done;
-  uint64_t q_full[2], q_empty[2], st_full[2], st_empty[2];
+  uint64_t kv_full, kv_empty, s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty;
+  uint64_t q_full[4], q_empty[4], do_full[4], do_empty[4];
 };
 
 template <int DT, int DH>
@@ -76,33 +86,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                         const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const BwdParams p) {
   using L = DkvSmem<DH>;
+  constexpr bool kEarly = DH == 64;
+  constexpr uint32_t kDp = kEarly ? 256 : 128, kDv = kDp + 128, kDk = kDv + DH;
   extern __shared__ uint8_t smem_raw[];
   __shared__ DkvBars bars;
+  __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  __shared__ AttnWork work;
-  __shared__ __align__(16) float st_lse[2][kAttnTile], st_delta[2][kAttnTile];
+  __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int kvh = blockIdx.x % p.hkv;
 
-  if (warp == 0) {
-    const AttnWork w = attn_find(p.rows, blockIdx.x / p.hkv, kAttnTile, false);
-    if (lane == 0) work = w;
-  } else if (warp == 8) {
+  if (warp == 8) {
     tmem_alloc_cta(&tmem_slot, 512);
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
+    attn_sched_init(sched, 11);
     mbar_init(&bars.kv_full, 1);
-    mbar_init(&bars.s_full, 1);
-    mbar_init(&bars.p_full, 8);
+    mbar_init(&bars.kv_empty, 1);
     mbar_init(&bars.dp_full, 1);
     mbar_init(&bars.ds_full, 8);
-    mbar_init(&bars.done, 1);
+    mbar_init(&bars.acc_full, 1);
+    mbar_init(&bars.acc_empty, 8);
+    mbar_init(&bars.st_full, 1);
+    mbar_init(&bars.st_empty, 8);
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.s_full[s], 1);
+      mbar_init(&bars.p_full[s], 8);
+    }
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&bars.q_full[s], 1);
       mbar_init(&bars.q_empty[s], 1);
-      mbar_init(&bars.st_full[s], 1);
-      mbar_init(&bars.st_empty[s], 8);
+      mbar_init(&bars.do_full[s], 1);
+      mbar_init(&bars.do_empty[s], 1);
     }
     fence_mbar_init();
   }
@@ -110,213 +125,270 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const AttnWork w = work;
-  if (w.tile < 0) {
-    attn_zero_gap(p.rows, w, p.dk, p.hkv, kvh, p.dim);
-    attn_zero_gap(p.rows, w, p.dv, p.hkv, kvh, p.dim);
-  } else {
-    const int nq = (w.len + kAttnTile - 1) / kAttnTile - w.tile;   // query tiles from the diagonal on
-    const int n = nq * p.group;
-    bool ok = true;
-    if (warp == 9) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
-        attn_load_tile<DH>(smem, &mk, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
-        attn_load_tile<DH>(smem + L::kTile, &mv, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
-        Ring r(2);
+  bool ok = true;
+  AttnWork w;
+  int kvh;
+  Ring rw(2);
+  auto q_tiles = [&]() { return (w.len + kAttnTile - 1) / kAttnTile - w.tile; };   // of a head, from the diagonal on
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 11) {
+      ok = attn_schedule(sched, p.rows, p.hkv, kAttnTile, false, [&](const AttnWork& g, int h) {
+        attn_zero_gap(p.rows, g, p.dk, p.hkv, h, p.dim);
+        attn_zero_gap(p.rows, g, p.dv, p.hkv, h, p.dim);
+      });
+    } else if (warp == 9) {
+      char *q_ring = smem + 2 * L::kTile, *do_ring = q_ring + L::kQ * L::kTile;
+      Ring rq(L::kQ), rd(L::kDo);
+      uint32_t used = 0;
+      while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
+        const int nq = q_tiles(), n = nq * p.group;
+        if (!warp_wait(&bars.kv_empty, (used & 1) ^ 1)) { ok = false; break; }
+        ++used;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
+          attn_load_tile<DH>(smem, &mk, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
+          attn_load_tile<DH>(smem + L::kTile, &mv, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
+        }
         int head = kvh * p.group, i = 0;
-        for (int it = 0; it < n; ++it, r.next()) {
-          if (!mbar_wait(&bars.q_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
-          mbar_arrive_expect_tx(&bars.q_full[r.idx], 2 * L::kTile);
-          char* dst = smem + (2 + 2 * r.idx) * L::kTile;
-          attn_load_tile<DH>(dst, &mq, &bars.q_full[r.idx], w.row + (w.tile + i) * kAttnTile, head, w.batch);
-          attn_load_tile<DH>(dst + L::kTile, &mdo, &bars.q_full[r.idx], w.row + (w.tile + i) * kAttnTile, head, w.batch);
+        for (int it = 0; it < n; ++it, rq.next(), rd.next()) {
+          const int row = w.row + (w.tile + i) * kAttnTile;
+          if (!warp_wait(&bars.q_empty[rq.idx], rq.phase ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.q_full[rq.idx], L::kTile);
+            attn_load_tile<DH>(q_ring + rq.idx * L::kTile, &mq, &bars.q_full[rq.idx], row, head, w.batch);
+          }
+          if (!warp_wait(&bars.do_empty[rd.idx], rd.phase ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.do_full[rd.idx], L::kTile);
+            attn_load_tile<DH>(do_ring + rd.idx * L::kTile, &mdo, &bars.do_full[rd.idx], row, head, w.batch);
+          }
           if (++i == nq) { i = 0; ++head; }
         }
       }
     } else if (warp == 10) {
-      Ring r(2);
-      int head = kvh * p.group, i = 0;
-      for (int it = 0; it < n; ++it, r.next()) {
-        const long long at = (long long)head * p.rows.rows + w.orow;
-        float a[4], b[4];
+      uint32_t cnt = 0;
+      while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
+        const int nq = q_tiles(), n = nq * p.group;
+        int head = kvh * p.group, i = 0;
+        for (int it = 0; it < n; ++it, ++cnt) {
+          const long long at = (long long)head * p.rows.rows + w.orow;
+          float a[4], b[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = (w.tile + i) * kAttnTile + e * 32 + lane;
-          a[e] = row < w.len ? __ldg(p.lse + at + row) : INFINITY;
-          b[e] = row < w.len ? __ldg(p.delta + at + row) : 0.f;
-        }
-        if (!warp_wait(&bars.st_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
+          for (int e = 0; e < 4; ++e) {
+            const int row = (w.tile + i) * kAttnTile + e * 32 + lane;
+            a[e] = row < w.len ? -__ldg(p.lse + at + row) : -INFINITY;
+            b[e] = row < w.len ? -__ldg(p.delta + at + row) : 0.f;
+          }
+          if (!warp_wait(&bars.st_empty, (cnt & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          st_lse[r.idx][e * 32 + lane] = a[e];
-          st_delta[r.idx][e * 32 + lane] = b[e];
+          for (int e = 0; e < 4; ++e) {
+            st_lse[e * 32 + lane] = a[e];
+            st_delta[e * 32 + lane] = b[e];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.st_full);
+          if (++i == nq) { i = 0; ++head; }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.st_full[r.idx]);
-        if (++i == nq) { i = 0; ++head; }
       }
     } else if (warp == 8) {
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t sk = smem_u32(smem), sv = sk + L::kTile, ring = sk + 2 * L::kTile;
-      const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DH;
-      int i = 0;   // query tile of the head
-      auto steps_of = [&](int tile) {
-        const int valid = w.len - (w.tile + tile) * kAttnTile;
-        return valid >= kAttnTile ? 8 : (valid + 15) >> 4;
-      };
-      auto arrived = [&](Ring& r, int tile) {   // the pair of tiles is there, and clean behind the sequence
-        if (!warp_wait(&bars.q_full[r.idx], r.phase)) return false;
-        const int valid = w.len - (w.tile + tile) * kAttnTile;
-        if (valid < kAttnTile) {
-          attn_zero_tail<DH>(smem + (2 + 2 * r.idx) * L::kTile, valid);
-          attn_zero_tail<DH>(smem + (3 + 2 * r.idx) * L::kTile, valid);
-        }
+      const uint32_t sk = smem_u32(smem), sv = sk + L::kTile, q_ring = sk + 2 * L::kTile, do_ring = q_ring + L::kQ * L::kTile;
+      Ring rq(L::kQ), rd(L::kDo);
+      uint32_t used = 0, cnt = 0;   // pieces of work; query tiles of all of them
+      int nq = 0;
+      // the tile is there, and clean behind the sequence
+      auto arrived = [&](uint64_t* full, uint32_t phase, uint32_t offset, int i) {
+        if (!warp_wait(full, phase)) return false;
+        const int valid = w.len - (w.tile + i) * kAttnTile;
+        if (valid < kAttnTile) attn_zero_tail<DH>(smem + offset, valid);
         tc_fence_after_sync();
         return true;
       };
-      Ring r(2);
-      ok = warp_wait(&bars.kv_full, 0) && arrived(r, 0);
-      if (ok && lane == 0) {
-        attn_mma_xyt<DH>(t_s, sk, ring, id_s);
-        umma_commit_cta(&bars.s_full);
-        attn_mma_xyt<DH>(t_dp, sv, ring + L::kTile, id_s);
-        umma_commit_cta(&bars.dp_full);
-      }
-      for (int it = 0; ok && it < n; ++it) {
-        const uint32_t q = ring + 2 * r.idx * L::kTile;
-        const int steps = steps_of(i);
-        Ring nx = r;
-        nx.next();
-        if (++i == nq) i = 0;
-        const bool more = it + 1 < n;
-        if (!warp_wait(&bars.p_full, it & 1)) { ok = false; break; }
-        tc_fence_after_sync();
-        if (lane == 0) attn_mma_py<DH>(t_dv, t_s, 64, q + L::kTile, id_o, it > 0, steps);
-        if (more) {
-          if (!arrived(nx, i)) { ok = false; break; }
-          if (lane == 0) {
-            attn_mma_xyt<DH>(t_s, sk, ring + 2 * nx.idx * L::kTile, id_s);
-            umma_commit_cta(&bars.s_full);
-          }
-        }
-        if (!warp_wait(&bars.ds_full, it & 1)) { ok = false; break; }
-        tc_fence_after_sync();
+      auto scores = [&](Ring& r, int i, uint32_t c) {
+        if (!arrived(&bars.q_full[r.idx], r.phase, (2 + r.idx) * L::kTile, i)) return false;
         if (lane == 0) {
-          attn_mma_py<DH>(t_dk, t_dp, 64, q, id_o, it > 0, steps);
-          umma_commit_cta(&bars.q_empty[r.idx]);
-          if (more) {
-            attn_mma_xyt<DH>(t_dp, sv, ring + (2 * nx.idx + 1) * L::kTile, id_s);
-            umma_commit_cta(&bars.dp_full);
-          } else {
-            umma_commit_cta(&bars.done);
-          }
+          const uint32_t b = kEarly ? (c & 1) : 0;
+          attn_mma_xyt<DH>(tmem + b * 128, sk, q_ring + r.idx * L::kTile, id_s);
+          umma_commit_cta(&bars.s_full[b]);
         }
-        r = nx;
+        return true;
+      };
+      auto dprobs = [&](Ring& r, int i, bool last) {
+        if (!arrived(&bars.do_full[r.idx], r.phase, (2 + L::kQ + r.idx) * L::kTile, i)) return false;
+        if (lane == 0) {
+          attn_mma_xyt<DH>(tmem + kDp, sv, do_ring + r.idx * L::kTile, id_s);
+          umma_commit_cta(&bars.dp_full);
+          if (last) umma_commit_cta(&bars.kv_empty);
+        }
+        return true;
+      };
+      while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
+        nq = q_tiles();
+        const int n = nq * p.group;
+        int i = 0;
+        ok = warp_wait(&bars.kv_full, used & 1) && scores(rq, 0, cnt) && dprobs(rd, 0, n == 1);
+        for (int it = 0; ok && it < n; ++it, ++cnt) {
+          const int valid = w.len - (w.tile + i) * kAttnTile;
+          const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
+          Ring nrq = rq, nrd = rd;
+          nrq.next();
+          nrd.next();
+          if (++i == nq) i = 0;
+          const bool more = it + 1 < n;
+          if (kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
+          const uint32_t dot = do_ring + rd.idx * L::kTile, pt = tmem + (kEarly ? (cnt & 1) * 128 : 0);
+          if (it == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (!warp_wait(&bars.p_full[c], cnt & 1)) { ok = false; break; }
+            tc_fence_after_sync();
+            if (lane == 0)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (h * 4 + c * 2 < steps)
+                  attn_mma_py<DH>(tmem + kDv, pt + h * 64 + c * 16, 0, dot + (h * 4 + c * 2) * 2048, id_o,
+                                  it > 0 || c > 0 || h > 0, min(2, steps - h * 4 - c * 2));
+          }
+          if (!ok) break;
+          if (lane == 0) umma_commit_cta(&bars.do_empty[rd.idx]);
+          if (!kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
+          if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (lane == 0) {
+            attn_mma_py<DH>(tmem + kDk, tmem + kDp, 64, q_ring + rq.idx * L::kTile, id_o, it > 0, steps);
+            umma_commit_cta(&bars.q_empty[rq.idx]);
+            if (!more) umma_commit_cta(&bars.acc_full);
+          }
+          if (more && !dprobs(nrd, i, it + 2 == n)) { ok = false; break; }
+          rq = nrq;
+          rd = nrd;
+        }
+        ++used;
       }
-    } else if (warp < 8) {
-      const int half = warp >> 2;   // which 64 query columns
-      const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-      const uint32_t s_addr = tmem + lanes + half * 64, dp_addr = s_addr + 128;
-      const int key = (warp & 3) * 32 + lane;
-      Ring r(2);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMathRegs));
+    const int half = warp >> 2;   // which 64 query columns
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t dp_addr = tmem + lanes + kDp + half * 64;
+    const int key = (warp & 3) * 32 + lane;
+    const float2 c2 = both(p.c);
+    const float4* lse = reinterpret_cast<const float4*>(st_lse + half * 64);
+    const float4* del = reinterpret_cast<const float4*>(st_delta + half * 64);
+    uint32_t cnt = 0, used = 0;
+    while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
+      const int nq = q_tiles(), n = nq * p.group;
       int i = 0;
-      const float2 c2 = make_float2(p.c, p.c);
-      for (int it = 0; it < n; ++it, r.next()) {
+      for (int it = 0; it < n; ++it, ++cnt) {
         const bool diag = i == 0;
         if (++i == nq) i = 0;
-        if (!warp_wait(&bars.st_full[r.idx], r.phase) || !warp_wait(&bars.s_full, it & 1)) { ok = false; break; }
+        const uint32_t b = kEarly ? (cnt & 1) : 0;
+        const uint32_t s_addr = tmem + lanes + b * 128 + half * 64;
+        if (!warp_wait(&bars.st_full, cnt & 1) || !warp_wait(&bars.s_full[b], kEarly ? (cnt >> 1) & 1 : cnt & 1)) { ok = false; break; }
         tc_fence_after_sync();
-        uint32_t s[64];
+        uint32_t s[64], pk[32];
         tmem_ld_x32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(s));
         tmem_ld_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_ld_wait();
-        const float4* lse = reinterpret_cast<const float4*>(st_lse[r.idx] + half * 64);
-        uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          const float4 z = lse[e >> 2];
-          const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, make_float2(-z.x, -z.y));
-          const float2 y = fma2(make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), c2, make_float2(-z.z, -z.w));
-          float v[4] = {ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y)};
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int e = c * 32; e < c * 32 + 32; e += 4) {
+            const float4 z = lse[e >> 2];
+            const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, make_float2(z.x, z.y));
+            const float2 y = fma2(make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), c2, make_float2(z.z, z.w));
+            s[e] = __float_as_uint(ex2(x.x));
+            s[e + 1] = __float_as_uint(ex2(x.y));
+            float2 q;
+            if ((e / 4) % PRISM_ATTN_BWD_POLY == PRISM_ATTN_BWD_POLY - 1) q = ex2_poly2(y);
+            else q = make_float2(ex2(y.x), ex2(y.y));
+            s[e + 2] = __float_as_uint(q.x);
+            s[e + 3] = __float_as_uint(q.y);
+          }
           if (diag) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
-              if (half * 64 + e + f < key) v[f] = 0.f;
+            for (int e = c * 32; e < c * 32 + 32; ++e)
+              if (half * 64 + e < key) s[e] = 0u;
           }
 #pragma unroll
-          for (int f = 0; f < 4; ++f) s[e + f] = __float_as_uint(v[f]);
-          pk[e >> 1] = Elem<DT>::pack(v[0], v[1]);
-          pk[(e >> 1) + 1] = Elem<DT>::pack(v[2], v[3]);
+          for (int e = c * 32; e < c * 32 + 32; e += 2)
+            pk[e >> 1] = Elem<DT>::pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+          tmem_st_x16(s_addr + c * 16, pk + c * 16);
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.p_full[c]);
         }
-        tmem_st_x32(s_addr, pk);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_full);
-        if (!warp_wait(&bars.dp_full, it & 1)) { ok = false; break; }
+        if (!warp_wait(&bars.dp_full, cnt & 1)) { ok = false; break; }
         tc_fence_after_sync();
-        const float4* del = reinterpret_cast<const float4*>(st_delta[r.idx] + half * 64);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t dp[32];
-          tmem_ld_x32(dp_addr + h * 32, dp);
+          tmem_ld_x32(dp_addr + c * 32, dp);
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float4 z = del[(h * 32 + e) >> 2];
-            const float zz[4] = {z.x, z.y, z.z, z.w};
-            float v[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              v[f] = __uint_as_float(s[h * 32 + e + f]) * (__uint_as_float(dp[e + f]) - zz[f]);
-              if (diag && half * 64 + h * 32 + e + f < key) v[f] = 0.f;
-            }
-            pk[(h * 32 + e) >> 1] = Elem<DT>::pack(v[0], v[1]);
-            pk[((h * 32 + e) >> 1) + 1] = Elem<DT>::pack(v[2], v[3]);
+            const float4 z = del[(c * 32 + e) >> 2];
+            float2 x = add2(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), make_float2(z.x, z.y));
+            float2 y = add2(make_float2(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), make_float2(z.z, z.w));
+            x = mul2(x, make_float2(__uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1])));
+            y = mul2(y, make_float2(__uint_as_float(s[c * 32 + e + 2]), __uint_as_float(s[c * 32 + e + 3])));
+            dp[e] = __float_as_uint(x.x); dp[e + 1] = __float_as_uint(x.y);
+            dp[e + 2] = __float_as_uint(y.x); dp[e + 3] = __float_as_uint(y.y);
           }
+          if (diag) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (half * 64 + c * 32 + e < key) dp[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            pk[(c * 32 + e) >> 1] = Elem<DT>::pack(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
         }
         tmem_st_x32(dp_addr, pk);
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars.st_empty[r.idx]);
+          mbar_arrive(&bars.st_empty);
           mbar_arrive(&bars.ds_full);
         }
       }
-      if (ok) {
-        if (warp_wait(&bars.done, 0)) {
-          tc_fence_after_sync();
-          const int row = w.tile * kAttnTile + key;
-          const bool mine = row < w.len;
-          const long long at = ((w.orow + row) * p.hkv + kvh) * p.dim;
-          if (half == 0) attn_store_row<DT, DH>(tmem + lanes + 256, 1.f, p.dv + at, p.dim, mine);
-          else attn_store_row<DT, DH>(tmem + lanes + 256 + DH, p.scale, p.dk + at, p.dim, mine);
-        } else {
-          ok = false;
-        }
-      }
+      if (!ok) break;
+      if (!warp_wait(&bars.acc_full, used & 1)) { ok = false; break; }
+      ++used;
+      tc_fence_after_sync();
+      const int row = w.tile * kAttnTile + key;
+      const bool mine = row < w.len;
+      const long long at = ((w.orow + row) * p.hkv + kvh) * p.dim;
+      if (half == 0) attn_store_row<DT, DH>(tmem + lanes + kDv, 1.f, p.dv + at, p.dim, mine);
+      else attn_store_row<DT, DH>(tmem + lanes + kDk, p.scale, p.dk + at, p.dim, mine);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.acc_empty);
     }
-    if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   }
+  if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 8) tmem_dealloc_cta(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------------------------------- dq
-// A query tile stays, key and value tiles stream by; two S buffers, so that the next scores are formed while the
-// warpgroups (64 key columns each) are in their exponentials.
+// A query tile stays, key and value tiles stream by.  S has one buffer, free again as soon as it is in registers; dP, over
+// which dS is written for dq += dS K, has two: the next tile's scores and dP are formed while the warpgroups (64 key
+// columns each) work on this one's.
 template <int DH>
 struct DqSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
-  static constexpr int kRing = 2;   // pairs of K and V tiles
-  static constexpr uint32_t kBytes = (2 + 2 * kRing) * kTile + 1024;
+  static constexpr int kK = DH == 128 ? 3 : 4, kV = DH == 128 ? 2 : 4;   // rings of K and of V tiles
+  static constexpr uint32_t kBytes = (2 + kK + kV) * kTile + 1024;
 };
 struct DqBars {
-  uint64_t q_full, s_full[2], dp_full, ds_full, done;
-  uint64_t k_full[2], v_full[2], kv_empty[2];
+  uint64_t q_full, q_empty, s_full, s_read, dp_full[2], ds_full, acc_full, acc_empty;
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
 template <int DT, int DH>
@@ -324,30 +396,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                        const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const BwdParams p) {
   using L = DqSmem<DH>;
+  constexpr uint32_t kDp = 128, kDq = 384;
   extern __shared__ uint8_t smem_raw[];
   __shared__ DqBars bars;
+  __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  __shared__ AttnWork work;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int head = blockIdx.x % p.hq, kvh = head / p.group;
 
-  if (warp == 0) {
-    const AttnWork w = attn_find(p.rows, blockIdx.x / p.hq, kAttnTile, true);
-    if (lane == 0) work = w;
-  } else if (warp == 8) {
+  if (warp == 8) {
     tmem_alloc_cta(&tmem_slot, 512);
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
+    attn_sched_init(sched, 10);
     mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.q_empty, 1);
+    mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.s_read, 8);
     mbar_init(&bars.ds_full, 8);
-    mbar_init(&bars.done, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.s_full[s], 1);
+    mbar_init(&bars.acc_full, 1);
+    mbar_init(&bars.acc_empty, 8);
+    mbar_init(&bars.dp_full[0], 1);
+    mbar_init(&bars.dp_full[1], 1);
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&bars.k_full[s], 1);
+      mbar_init(&bars.k_empty[s], 1);
       mbar_init(&bars.v_full[s], 1);
-      mbar_init(&bars.kv_empty[s], 1);
+      mbar_init(&bars.v_empty[s], 1);
     }
     fence_mbar_init();
   }
@@ -355,96 +430,127 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const AttnWork w = work;
-  if (w.tile < 0) {
-    attn_zero_gap(p.rows, w, p.dq, p.hq, head, p.dim);
-  } else {
-    const int n = w.tile + 1;   // key tiles up to the diagonal
-    bool ok = true;
-    if (warp == 9) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
-        attn_load_tile<DH>(smem, &mq, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
-        attn_load_tile<DH>(smem + L::kTile, &mdo, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
-        Ring r(2);
-        for (int j = 0; j < n; ++j, r.next()) {
-          if (!mbar_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
-          char* dst = smem + (2 + 2 * r.idx) * L::kTile;
-          mbar_arrive_expect_tx(&bars.k_full[r.idx], L::kTile);
-          attn_load_tile<DH>(dst, &mk, &bars.k_full[r.idx], w.row + j * kAttnTile, kvh, w.batch);
-          mbar_arrive_expect_tx(&bars.v_full[r.idx], L::kTile);
-          attn_load_tile<DH>(dst + L::kTile, &mv, &bars.v_full[r.idx], w.row + j * kAttnTile, kvh, w.batch);
+  bool ok = true;
+  AttnWork w;
+  int head;
+  Ring rw(2);
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 11) {
+      ok = attn_schedule(sched, p.rows, p.hq, kAttnTile, true,
+                         [&](const AttnWork& g, int h) { attn_zero_gap(p.rows, g, p.dq, p.hq, h, p.dim); });
+    } else if (warp == 9) {
+      char *k_ring = smem + 2 * L::kTile, *v_ring = k_ring + L::kK * L::kTile;
+      Ring rk(L::kK), rv(L::kV);
+      uint32_t used = 0;
+      while (ok && attn_next(sched, rw, &w, &head, &ok)) {
+        const int kvh = head / p.group;
+        if (!warp_wait(&bars.q_empty, (used & 1) ^ 1)) { ok = false; break; }
+        ++used;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
+          attn_load_tile<DH>(smem, &mq, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
+          attn_load_tile<DH>(smem + L::kTile, &mdo, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
+        }
+        for (int j = 0; j <= w.tile; ++j, rk.next(), rv.next()) {
+          if (!warp_wait(&bars.k_empty[rk.idx], rk.phase ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.k_full[rk.idx], L::kTile);
+            attn_load_tile<DH>(k_ring + rk.idx * L::kTile, &mk, &bars.k_full[rk.idx], w.row + j * kAttnTile, kvh, w.batch);
+          }
+          if (!warp_wait(&bars.v_empty[rv.idx], rv.phase ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.v_full[rv.idx], L::kTile);
+            attn_load_tile<DH>(v_ring + rv.idx * L::kTile, &mv, &bars.v_full[rv.idx], w.row + j * kAttnTile, kvh, w.batch);
+          }
         }
       }
     } else if (warp == 8) {
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t sq = smem_u32(smem), sdo = sq + L::kTile, ring = sq + 2 * L::kTile;
-      const uint32_t t_dp = tmem + 256, t_dq = tmem + 384;
-      Ring r(2);
-      auto scores = [&](Ring& rr, int j) {
-        if (!warp_wait(&bars.k_full[rr.idx], rr.phase)) return false;
+      const uint32_t sq = smem_u32(smem), sdo = sq + L::kTile, k_ring = sq + 2 * L::kTile, v_ring = k_ring + L::kK * L::kTile;
+      Ring rk(L::kK), rs(L::kK), rv(L::kV);   // key tiles of dq and of the scores (one ahead), value tiles
+      uint32_t used = 0, cnt = 0;
+      auto scores = [&](int j, uint32_t c) {
+        if (!warp_wait(&bars.k_full[rs.idx], rs.phase) || !warp_wait(&bars.s_read, (c & 1) ^ 1)) return false;
         const int valid = w.len - j * kAttnTile;
-        if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + 2 * rr.idx) * L::kTile, valid);
+        if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rs.idx) * L::kTile, valid);
         tc_fence_after_sync();
         if (lane == 0) {
-          attn_mma_xyt<DH>(tmem + (j & 1) * 128, sq, ring + 2 * rr.idx * L::kTile, id_s);
-          umma_commit_cta(&bars.s_full[j & 1]);
+          attn_mma_xyt<DH>(tmem, sq, k_ring + rs.idx * L::kTile, id_s);
+          umma_commit_cta(&bars.s_full);
         }
+        rs.next();
         return true;
       };
-      auto dprobs = [&](Ring& rr) {
-        if (!warp_wait(&bars.v_full[rr.idx], rr.phase)) return false;
+      auto dprobs = [&](uint32_t c, bool last) {
+        if (!warp_wait(&bars.v_full[rv.idx], rv.phase)) return false;
         tc_fence_after_sync();
         if (lane == 0) {
-          attn_mma_xyt<DH>(t_dp, sdo, ring + (2 * rr.idx + 1) * L::kTile, id_s);
-          umma_commit_cta(&bars.dp_full);
+          attn_mma_xyt<DH>(tmem + kDp + (c & 1) * 128, sdo, v_ring + rv.idx * L::kTile, id_s);
+          umma_commit_cta(&bars.dp_full[c & 1]);
+          umma_commit_cta(&bars.v_empty[rv.idx]);
+          if (last) umma_commit_cta(&bars.q_empty);
         }
+        rv.next();
         return true;
       };
-      ok = warp_wait(&bars.q_full, 0) && scores(r, 0) && dprobs(r);
-      for (int j = 0; ok && j < n; ++j) {
-        Ring nx = r;
-        nx.next();
-        const bool more = j + 1 < n;
-        if (more && !scores(nx, j + 1)) { ok = false; break; }
-        if (!warp_wait(&bars.ds_full, j & 1)) { ok = false; break; }
-        tc_fence_after_sync();
-        const int valid = w.len - j * kAttnTile;
-        if (lane == 0) {
-          attn_mma_py<DH>(t_dq, t_dp, 64, ring + 2 * r.idx * L::kTile, id_o, j > 0, valid >= kAttnTile ? 8 : (valid + 15) >> 4);
-          umma_commit_cta(&bars.kv_empty[r.idx]);
-          if (!more) umma_commit_cta(&bars.done);
+      while (ok && attn_next(sched, rw, &w, &head, &ok)) {
+        const int n = w.tile + 1;   // key tiles up to the diagonal
+        ok = warp_wait(&bars.q_full, used & 1) && scores(0, cnt) && dprobs(cnt, n == 1);
+        for (int j = 0; ok && j < n; ++j, ++cnt) {
+          const bool more = j + 1 < n;
+          if (more && !(scores(j + 1, cnt + 1) && dprobs(cnt + 1, j + 2 == n))) { ok = false; break; }
+          if (j == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
+          if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          const int valid = w.len - j * kAttnTile;
+          if (lane == 0) {
+            attn_mma_py<DH>(tmem + kDq, tmem + kDp + (cnt & 1) * 128, 64, k_ring + rk.idx * L::kTile, id_o, j > 0,
+                            valid >= kAttnTile ? 8 : (valid + 15) >> 4);
+            umma_commit_cta(&bars.k_empty[rk.idx]);
+            if (!more) umma_commit_cta(&bars.acc_full);
+          }
+          rk.next();
         }
-        if (more && !dprobs(nx)) { ok = false; break; }
-        r = nx;
+        ++used;
       }
-    } else if (warp < 8) {
-      const int half = warp >> 2;   // which 64 key columns
-      const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-      const uint32_t dp_addr = tmem + lanes + 256 + half * 64;
-      const int r = (warp & 3) * 32 + lane;
-      const int row = w.tile * kAttnTile + r;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMathRegs));
+    const int half = warp >> 2;   // which 64 key columns
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t s_addr = tmem + lanes + half * 64;
+    const int r = (warp & 3) * 32 + lane;
+    const float2 c2 = both(p.c);
+    uint32_t cnt = 0, used = 0;
+    while (ok && attn_next(sched, rw, &w, &head, &ok)) {
+      const int n = w.tile + 1, row = w.tile * kAttnTile + r;
       const bool mine = row < w.len;
       const long long at = (long long)head * p.rows.rows + w.orow + row;
-      const float neg = mine ? -__ldg(p.lse + at) : -INFINITY, delta = mine ? __ldg(p.delta + at) : 0.f;
-      const float2 c2 = make_float2(p.c, p.c), n2 = make_float2(neg, neg);
-      for (int j = 0; j < n; ++j) {
-        const bool diag = j + 1 == n;
-        if (!warp_wait(&bars.s_full[j & 1], (j >> 1) & 1)) { ok = false; break; }
+      const float2 n2 = both(mine ? -__ldg(p.lse + at) : -INFINITY), d2 = both(mine ? -__ldg(p.delta + at) : 0.f);
+      for (int j = 0; j < n; ++j, ++cnt) {
+        if (!warp_wait(&bars.s_full, cnt & 1)) { ok = false; break; }
         tc_fence_after_sync();
-        const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + half * 64;
         uint32_t s[64];
         tmem_ld_x32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(s));
         tmem_ld_x32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.s_read);
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
           const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, n2);
-          s[e] = __float_as_uint(ex2(x.x));
-          s[e + 1] = __float_as_uint(ex2(x.y));
+          float2 q;
+          if ((e / 2) % (2 * PRISM_ATTN_BWD_POLY) == 2 * PRISM_ATTN_BWD_POLY - 1) q = ex2_poly2(x);
+          else q = make_float2(ex2(x.x), ex2(x.y));
+          s[e] = __float_as_uint(q.x);
+          s[e + 1] = __float_as_uint(q.y);
         }
-        if (!warp_wait(&bars.dp_full, j & 1)) { ok = false; break; }
+        if (!warp_wait(&bars.dp_full[cnt & 1], (cnt >> 1) & 1)) { ok = false; break; }
         tc_fence_after_sync();
+        const uint32_t dp_addr = tmem + lanes + kDp + (cnt & 1) * 128 + half * 64;
         uint32_t pk[32];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -453,14 +559,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float a = __uint_as_float(s[h * 32 + e]) * (__uint_as_float(dp[e]) - delta);
-            float b = __uint_as_float(s[h * 32 + e + 1]) * (__uint_as_float(dp[e + 1]) - delta);
-            if (diag) {
-              if (half * 64 + h * 32 + e > r) a = 0.f;
-              if (half * 64 + h * 32 + e + 1 > r) b = 0.f;
-            }
-            pk[(h * 32 + e) >> 1] = Elem<DT>::pack(a, b);
+            const float2 x = mul2(add2(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), d2),
+                                  make_float2(__uint_as_float(s[h * 32 + e]), __uint_as_float(s[h * 32 + e + 1])));
+            dp[e] = __float_as_uint(x.x);
+            dp[e + 1] = __float_as_uint(x.y);
           }
+          if (j + 1 == n) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (half * 64 + h * 32 + e > r) dp[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            pk[(h * 32 + e) >> 1] = Elem<DT>::pack(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
         }
         tmem_st_x32(dp_addr, pk);
         tmem_st_wait();
@@ -468,18 +579,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.ds_full);
       }
-      if (ok) {
-        if (warp_wait(&bars.done, 0)) {
-          tc_fence_after_sync();
-          if (half == 0)
-            attn_store_row<DT, DH>(tmem + lanes + 384, p.scale, p.dq + ((w.orow + row) * p.hq + head) * p.dim, p.dim, mine);
-        } else {
-          ok = false;
-        }
-      }
+      if (!ok) break;
+      if (!warp_wait(&bars.acc_full, used & 1)) { ok = false; break; }
+      ++used;
+      tc_fence_after_sync();
+      uint16_t* dst = p.dq + ((w.orow + row) * p.hq + head) * p.dim;
+      // each warpgroup half of the features
+      if (half * (DH / 2) < p.dim)
+        attn_store_row<DT, DH / 2>(tmem + lanes + kDq + half * (DH / 2), p.scale, dst + half * (DH / 2), p.dim - half * (DH / 2), mine);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.acc_empty);
     }
-    if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   }
+  if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 8) tmem_dealloc_cta(tmem, 512);

@@ -1,11 +1,14 @@
 // Causal attention, forward: o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j for every head of every sequence.
 //
 // One pass over the keys with a running maximum m and sum l per row (exponents in base 2, c = scale log2 e):
-//   S = Q K^T (tcgen05, fp32 in TMEM) -> p = 2^(c s - c m) (registers, one row a thread) -> 16 bits, into TMEM over S
+//   S = Q K^T (tcgen05, fp32 in TMEM) -> p = 2^(c s - c m) (registers, one row a thread) -> 16 bits, into TMEM
 //   -> O += P V (tcgen05, P from TMEM);  O and l are rescaled only when a row's maximum has grown by more than 2^8
-// (every p stays below 2^8, exactly representable headroom in both 16-bit types); the end divides by l.
-// A CTA owns 256 rows of a head as two 128-row tiles with a warpgroup each: while one warpgroup is in its
-// exponentials, the tensor core works on the other's products.  Keys and values pass through one ring of shared tiles.
+// (every p stays below 2^8, which costs neither 16-bit type any of its digits); the end divides by l.
+// A CTA works on two 128-row tiles at a time with a warpgroup each (two heads of a group, whose keys are the same, or 256
+// rows of one head), so that the tensor core has the other tile's products while a warpgroup is in its exponentials.
+// P is handed over in halves: the first half's product runs beside the second half's exponentials.  Keys and values pass
+// through one ring of shared tiles.  TMEM, heads of up to 64: S of both tiles, P of both, O of both, so that the next
+// scores are formed as soon as these have been read; wider heads: P takes the place of S, which waits for P V.
 #include "prism_attn.cuh"
 #include "prism_host.cuh"
 #include "prism_attn_host.cuh"
@@ -18,11 +21,15 @@ struct FwdParams {
   uint16_t* o;     // rows x heads x dim
   float* lse;      // heads x rows, c m + log2 l per row, or null
   int hq, group, dim;
+  int pair;        // 1: the two tiles are the same rows of two heads; 0: 256 rows of one head
   float c;         // scale * log2 e
   int* err;
 };
 
-constexpr int kThreads = 320;   // two softmax warpgroups, the MMA warp, the TMA warp
+// Two softmax warpgroups, and one of the MMA warp, the TMA warp, the warp that looks for work and one that only lends its
+// registers: a softmax thread holds a row of 128 scores.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is
+// launched with.
+constexpr int kThreads = 384, kSoftmaxRegs = 208, kOtherRegs = 88;
 
 template <int DH>
 struct FwdSmem {
@@ -32,35 +39,64 @@ struct FwdSmem {
 };
 
 struct FwdBars {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
   uint64_t kv_full[10], kv_empty[10];
 };
+
+// The two tiles of a piece of work: row offset, head and number of key blocks.
+struct FwdTiles {
+  int row[2], head[2], n[2];
+  __device__ __forceinline__ FwdTiles(const FwdParams& p, const AttnWork& w, int slot_head) {
+    if (p.pair) {
+      row[0] = row[1] = w.tile * kAttnTile;
+      head[0] = 2 * slot_head;
+      head[1] = 2 * slot_head + 1;
+      n[0] = n[1] = w.tile + 1;
+    } else {
+      row[0] = 2 * w.tile * kAttnTile;
+      row[1] = row[0] + kAttnTile;
+      head[0] = head[1] = slot_head;
+      n[0] = 2 * w.tile + 1;
+      n[1] = w.len > row[1] ? n[0] + 1 : 0;
+    }
+  }
+  __device__ __forceinline__ int most() const { return max(n[0], n[1]); }
+};
+
+// Every kPolyOf-th pair of exponentials goes to the FMA pipe.
+#ifndef PRISM_ATTN_FWD_POLY
+#define PRISM_ATTN_FWD_POLY 4
+#endif
 
 template <int DT, int DH>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                     const __grid_constant__ CUtensorMap mv, const FwdParams p) {
   using L = FwdSmem<DH>;
+  constexpr bool kEarly = DH == 64;   // S does not share its columns with P
+  constexpr uint32_t kO = kEarly ? 384 : 256;
   extern __shared__ uint8_t smem_raw[];
   __shared__ FwdBars bars;
+  __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  __shared__ AttnWork work;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int head = blockIdx.x % p.hq, kvh = head / p.group;
 
-  if (warp == 0) {
-    const AttnWork w = attn_find(p.rows, blockIdx.x / p.hq, 2 * kAttnTile, true);
-    if (lane == 0) work = w;
-  } else if (warp == 8) {
+  if (warp == 8) {
     tmem_alloc_cta(&tmem_slot, 512);
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
+    attn_sched_init(sched, 10);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bars.q_full[t], 1);
+      mbar_init(&bars.q_empty[t], 1);
       mbar_init(&bars.s_full[t], 1);
-      mbar_init(&bars.p_full[t], 4);
+      mbar_init(&bars.s_read[t], 4);
+      mbar_init(&bars.p_full[t][0], 4);
+      mbar_init(&bars.p_full[t][1], 4);
+      mbar_init(&bars.pv_done[t], 1);
       mbar_init(&bars.o_full[t], 1);
+      mbar_init(&bars.o_empty[t], 4);
     }
     for (int s = 0; s < L::kRing; ++s) {
       mbar_init(&bars.kv_full[s], 1);
@@ -72,108 +108,174 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const AttnWork w = work;
+  bool ok = true;
+  AttnWork w;
+  int slot_head;
+  Ring rw(2);
 
-  if (w.tile < 0) {
-    attn_zero_gap(p.rows, w, p.o, p.hq, head, p.dim);
-  } else {
-    const int m0 = w.tile * 2 * kAttnTile;
-    const int n0 = 2 * w.tile + 1;                                   // key blocks of the first tile ...
-    const int n1 = w.len > m0 + kAttnTile ? n0 + 1 : 0;              // ... and of the second, which may be empty
-    const int n = max(n0, n1);
-    bool ok = true;
-    if (warp == 9) {
-      if (lane == 0) {
-        char* ring = smem + 2 * L::kTile;
-        for (int t = 0; t < (n1 ? 2 : 1); ++t) {
-          mbar_arrive_expect_tx(&bars.q_full[t], L::kTile);
-          attn_load_tile<DH>(smem + t * L::kTile, &mq, &bars.q_full[t], w.row + m0 + t * kAttnTile, head, w.batch);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 11) {
+      ok = attn_schedule(sched, p.rows, p.pair ? p.hq / 2 : p.hq, p.pair ? kAttnTile : 2 * kAttnTile, true,
+                         [&](const AttnWork& g, int h) {
+                           for (int t = 0; t <= p.pair; ++t) attn_zero_gap(p.rows, g, p.o, p.hq, p.pair ? 2 * h + t : h, p.dim);
+                         });
+    } else if (warp == 9) {
+      char* ring = smem + 2 * L::kTile;
+      Ring r(L::kRing);
+      uint32_t used[2] = {0, 0};   // pieces of work that tile t had a part in
+      while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
+        const FwdTiles tl(p, w, slot_head);
+        for (int t = 0; t < 2; ++t) {
+          if (tl.n[t] == 0) continue;
+          if (!warp_wait(&bars.q_empty[t], (used[t] & 1) ^ 1)) { ok = false; break; }
+          ++used[t];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.q_full[t], L::kTile);
+            attn_load_tile<DH>(smem + t * L::kTile, &mq, &bars.q_full[t], w.row + tl.row[t], tl.head[t], w.batch);
+          }
         }
-        Ring r(L::kRing);
-        for (int i = 0; i < 2 * n; ++i, r.next()) {
-          if (!mbar_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
-          mbar_arrive_expect_tx(&bars.kv_full[r.idx], L::kTile);
-          attn_load_tile<DH>(ring + r.idx * L::kTile, (i & 1) ? &mv : &mk, &bars.kv_full[r.idx],
-                             w.row + (i >> 1) * kAttnTile, kvh, w.batch);
+        const int n = tl.most(), kvh = tl.head[0] / p.group;
+        for (int i = 0; ok && i < 2 * n; ++i, r.next()) {
+          if (!warp_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.kv_full[r.idx], L::kTile);
+            attn_load_tile<DH>(ring + r.idx * L::kTile, (i & 1) ? &mv : &mk, &bars.kv_full[r.idx],
+                               w.row + (i >> 1) * kAttnTile, kvh, w.batch);
+          }
         }
       }
     } else if (warp == 8) {
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
       const uint32_t ring = smem_u32(smem) + 2 * L::kTile;
-      Ring rk(L::kRing), rv(L::kRing);
-      rv.next();
-      auto next2 = [](Ring& r) { r.next(); r.next(); };
+      Ring rk(L::kRing);
+      uint32_t used[2] = {0, 0}, made[2] = {0, 0}, blocks[2] = {0, 0};   // work, scores and key blocks of tile t so far
       // every lane waits (the warp stays together for the zeros of a last tile), one issues
-      if (!warp_wait(&bars.kv_full[0], 0)) ok = false;
-      for (int t = 0; ok && t < (n1 ? 2 : 1); ++t) {
-        if (!warp_wait(&bars.q_full[t], 0)) { ok = false; break; }
+      auto scores = [&](int t, uint32_t k_tile, bool last) {
         tc_fence_after_sync();
         if (lane == 0) {
-          attn_mma_xyt<DH>(tmem + t * 128, smem_u32(smem) + t * L::kTile, ring, id_s);
+          attn_mma_xyt<DH>(tmem + t * 128, smem_u32(smem) + t * L::kTile, k_tile, id_s);
           umma_commit_cta(&bars.s_full[t]);
+          if (last) umma_commit_cta(&bars.q_empty[t]);
         }
-      }
-      if (ok && lane == 0) umma_commit_cta(&bars.kv_empty[0]);
-      next2(rk);
-      for (int j = 0; ok && j < n; ++j) {
-        if (!warp_wait(&bars.kv_full[rv.idx], rv.phase)) { ok = false; break; }
-        const int valid = w.len - j * kAttnTile;
-        if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rv.idx) * L::kTile, valid);
-        const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
-        const bool more = j + 1 < n;
-        if (more && !warp_wait(&bars.kv_full[rk.idx], rk.phase)) { ok = false; break; }
-        for (int t = 0; t < 2; ++t) {
-          const int nt = t ? n1 : n0;
-          if (j >= nt) continue;
-          if (!warp_wait(&bars.p_full[t], j & 1)) { ok = false; break; }
-          tc_fence_after_sync();
-          if (lane == 0) {
-            attn_mma_py<DH>(tmem + 256 + t * DH, tmem + t * 128, 32, ring + rv.idx * L::kTile, id_o, j > 0, steps);
-            if (j + 1 == nt) umma_commit_cta(&bars.o_full[t]);
-            if (j + 1 < nt) {
-              attn_mma_xyt<DH>(tmem + t * 128, smem_u32(smem) + t * L::kTile, ring + rk.idx * L::kTile, id_s);
-              umma_commit_cta(&bars.s_full[t]);
+        ++made[t];
+      };
+      while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
+        const FwdTiles tl(p, w, slot_head);
+        const int n = tl.most();
+        Ring rv = rk;
+        rv.next();
+        ok = warp_wait(&bars.kv_full[rk.idx], rk.phase);
+        for (int t = 0; ok && t < 2; ++t) {
+          if (tl.n[t] == 0) continue;
+          if (!warp_wait(&bars.q_full[t], used[t] & 1)) { ok = false; break; }
+          // the scores of the work before have been read (where P took their place, its product came after)
+          if (kEarly && !warp_wait(&bars.s_read[t], (made[t] & 1) ^ 1)) { ok = false; break; }
+          scores(t, ring + rk.idx * L::kTile, tl.n[t] == 1);
+        }
+        if (ok && lane == 0) umma_commit_cta(&bars.kv_empty[rk.idx]);
+        rk.next();
+        rk.next();
+        for (int j = 0; ok && j < n; ++j) {
+          const bool more = j + 1 < n;
+          if (more && !warp_wait(&bars.kv_full[rk.idx], rk.phase)) { ok = false; break; }
+          if (kEarly && more) {
+            for (int t = 0; t < 2; ++t) {
+              if (j + 1 >= tl.n[t]) continue;
+              if (!warp_wait(&bars.s_read[t], (made[t] & 1) ^ 1)) { ok = false; break; }
+              scores(t, ring + rk.idx * L::kTile, j + 2 == tl.n[t]);
             }
+            if (!ok) break;
+            if (lane == 0) umma_commit_cta(&bars.kv_empty[rk.idx]);
           }
+          if (!warp_wait(&bars.kv_full[rv.idx], rv.phase)) { ok = false; break; }
+          const int valid = w.len - j * kAttnTile;
+          if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rv.idx) * L::kTile, valid);
+          const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
+          const uint32_t v_tile = ring + rv.idx * L::kTile;
+          for (int t = 0; t < 2; ++t) {
+            if (j >= tl.n[t]) continue;
+            const uint32_t pt = kEarly ? tmem + 256 + t * 64 : tmem + t * 128;
+            if (j == 0 && !warp_wait(&bars.o_empty[t], (used[t] & 1) ^ 1)) { ok = false; break; }
+            if (!warp_wait(&bars.p_full[t][0], blocks[t] & 1)) { ok = false; break; }
+            tc_fence_after_sync();
+            if (lane == 0) attn_mma_py<DH>(tmem + kO + t * DH, pt, 32, v_tile, id_o, j > 0, min(steps, 4));
+            if (!warp_wait(&bars.p_full[t][1], blocks[t] & 1)) { ok = false; break; }
+            tc_fence_after_sync();
+            if (lane == 0) {
+              if (steps > 4) attn_mma_py<DH>(tmem + kO + t * DH, pt + 32, 32, v_tile + 4 * 2048, id_o, true, steps - 4);
+              if (j + 1 == tl.n[t]) umma_commit_cta(&bars.o_full[t]);
+              else if (kEarly) umma_commit_cta(&bars.pv_done[t]);
+            }
+            if (!kEarly && j + 1 < tl.n[t]) scores(t, ring + rk.idx * L::kTile, j + 2 == tl.n[t]);
+            ++blocks[t];
+          }
+          if (!ok) break;
+          if (lane == 0) {
+            umma_commit_cta(&bars.kv_empty[rv.idx]);
+            if (!kEarly && more) umma_commit_cta(&bars.kv_empty[rk.idx]);
+          }
+          if (more) {
+            rk.next();
+            rk.next();
+          }
+          rv.next();
+          rv.next();
         }
-        if (!ok) break;
-        if (lane == 0) {
-          umma_commit_cta(&bars.kv_empty[rv.idx]);
-          if (more) umma_commit_cta(&bars.kv_empty[rk.idx]);
-        }
-        next2(rv);
-        next2(rk);
+        for (int t = 0; t < 2; ++t) used[t] += tl.n[t] > 0;
       }
-    } else {
-      const int t = warp >> 2;
-      const int nt = t ? n1 : n0;
-      const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-      const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + 256 + t * DH;
-      const int r = (warp & 3) * 32 + lane;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + kO + t * DH;
+    const uint32_t p_addr = kEarly ? tmem + lanes + 256 + t * 64 : s_addr;
+    const int r = (warp & 3) * 32 + lane;
+    uint32_t phase = 0, used = 0, pv = 0;
+    while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
+      const FwdTiles tl(p, w, slot_head);
+      const int nt = tl.n[t];
+      if (nt == 0) continue;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < nt; ++j) {
-        if (!warp_wait(&bars.s_full[t], j & 1)) { ok = false; break; }
+      for (int j = 0; j < nt; ++j, phase ^= 1u) {
+        if (!warp_wait(&bars.s_full[t], phase)) { ok = false; break; }
         tc_fence_after_sync();
         uint32_t s[128];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld_x32(s_addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
         tmem_ld_wait();
+        if (kEarly) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_read[t]);
+        }
         if (j + 1 == nt) {   // the tile's own rows: keys up to the row itself
 #pragma unroll
           for (int e = 0; e < 128; ++e)
             if (e > r) s[e] = 0xff800000u;
         }
-        float mx0 = __uint_as_float(s[0]), mx1 = __uint_as_float(s[1]);
+        float mx[8];
 #pragma unroll
-        for (int e = 2; e < 128; e += 4) {
-          mx0 = max3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-          if (e + 3 < 128) mx1 = max3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+        for (int e = 0; e < 8; ++e) mx[e] = max_nan(__uint_as_float(s[e]), __uint_as_float(s[e + 8]));
+#pragma unroll
+        for (int e = 16; e < 128; e += 16)
+#pragma unroll
+          for (int f = 0; f < 8; ++f)
+            mx[f] = max3_nan(mx[f], __uint_as_float(s[e + f]), __uint_as_float(s[e + 8 + f]));
+        const float mnew = max3_nan(max3_nan(m, mx[0], mx[1]), max3_nan(mx[2], mx[3], mx[4]), max3_nan(mx[5], mx[6], mx[7]));
+        // P V of the block before is done: its P may be written over and O rescaled.  (Where S waits for that product, the
+        // scores' arrival says so.)
+        if (kEarly && j > 0) {
+          if (!warp_wait(&bars.pv_done[t], pv & 1)) { ok = false; break; }
+          ++pv;
+          tc_fence_after_sync();
         }
-        const float mx = max3(m, mx0, mx1);
-        // (two rows at -infinity: the difference is NaN and nothing is rescaled, there is nothing yet)
-        if (__any_sync(0xffffffffu, (mx - m) * p.c > 8.f)) {
-          const float f = ex2((m - (mx == -INFINITY ? 0.f : mx)) * p.c);
-          m = mx;
+        // (a NaN among the scores makes the comparison fail and m NaN: the whole row is NaN then.  A row at -infinity
+        // has NaN on its left side as well, and nothing to rescale.)
+        if (__any_sync(0xffffffffu, !((mnew - m) * p.c <= 8.f))) {
+          const float f = ex2((m - (mnew == -INFINITY ? 0.f : mnew)) * p.c);
+          m = mnew;
           l *= f;
           if (j > 0) {
 #pragma unroll
@@ -187,41 +289,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float2 c2 = make_float2(p.c, p.c);
-        const float neg = m == -INFINITY ? 0.f : -m * p.c;
-        const float2 n2 = make_float2(neg, neg);
-        float l0 = 0.f, l1 = 0.f;
-        uint32_t* pk = s;   // pairs land in the first half of the registers
+        const float2 c2 = both(p.c), n2 = both(m == -INFINITY ? 0.f : -m * p.c);
+        float2 sum0 = both(0.f), sum1 = both(0.f);
 #pragma unroll
-        for (int e = 0; e < 128; e += 2) {
-          const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, n2);
-          const float a = ex2(x.x), b = ex2(x.y);
-          l0 += a;
-          l1 += b;
-          pk[e >> 1] = Elem<DT>::pack(a, b);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t* pk = s + h * 32;   // pairs land in the first half of the registers
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(s[h * 64 + e]), __uint_as_float(s[h * 64 + e + 1])), c2, n2);
+            float2 y;
+            if ((e / 2) % PRISM_ATTN_FWD_POLY == PRISM_ATTN_FWD_POLY - 1) y = ex2_poly2(x);
+            else y = make_float2(ex2(x.x), ex2(x.y));
+            if (e & 2) sum1 = add2(sum1, y);
+            else sum0 = add2(sum0, y);
+            pk[e >> 1] = Elem<DT>::pack(y.x, y.y);
+          }
+          tmem_st_x32(p_addr + h * 32, pk);
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.p_full[t][h]);
         }
-        l += l0 + l1;
-        tmem_st_x32(s_addr, pk);
-        tmem_st_x32(s_addr + 32, pk + 32);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_full[t]);
+        sum0 = add2(sum0, sum1);
+        l += sum0.x + sum0.y;
       }
-      if (ok && nt > 0) {
-        if (warp_wait(&bars.o_full[t], 0)) {
-          tc_fence_after_sync();
-          const int row = m0 + t * kAttnTile + r;
-          const bool mine = row < w.len;
-          attn_store_row<DT, DH>(o_addr, 1.f / l, p.o + ((w.orow + row) * p.hq + head) * p.dim, p.dim, mine);
-          if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + lg2(l);
-        } else {
-          ok = false;
-        }
-      }
+      if (!ok) break;
+      if (!warp_wait(&bars.o_full[t], used & 1)) { ok = false; break; }
+      ++used;
+      tc_fence_after_sync();
+      const int row = tl.row[t] + r, head = tl.head[t];
+      const bool mine = row < w.len;
+      attn_store_row<DT, DH>(o_addr, 1.f / l, p.o + ((w.orow + row) * p.hq + head) * p.dim, p.dim, mine);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.o_empty[t]);
+      if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + lg2(l);
     }
-    if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   }
+  if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 8) tmem_dealloc_cta(tmem, 512);
@@ -231,7 +336,8 @@ template <int DT, int DH>
 int launch_t(const AttnArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p) {
   auto* kern = attn_fwd_kernel<DT, DH>;
   if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), FwdSmem<DH>::kBytes, "causal attention")) return rc;
-  kern<<<(unsigned)p.rows.tiles * (unsigned)a.hq, kThreads, FwdSmem<DH>::kBytes, a.stream>>>(mq, mk, mv, p);
+  const unsigned heads = (unsigned)(p.pair ? a.hq / 2 : a.hq);
+  kern<<<(unsigned)p.rows.tiles * heads, kThreads, FwdSmem<DH>::kBytes, a.stream>>>(mq, mk, mv, p);
   return check_launch("causal attention");
 }
 
@@ -239,11 +345,12 @@ int launch_t(const AttnArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, co
 
 int launch_attn_fwd(const AttnArgs& a) {
   FwdParams p;
-  if (int rc = attn_rows(a, 2 * kAttnTile, a.hq, &p.rows)) return rc;
+  p.hq = a.hq; p.group = a.hq / a.hkv; p.dim = a.dim;
+  p.pair = p.group % 2 == 0;
+  if (int rc = attn_rows(a, p.pair ? kAttnTile : 2 * kAttnTile, a.hq, &p.rows)) return rc;
   if (p.rows.tiles == 0) return PRISM_OK;
   p.o = static_cast<uint16_t*>(a.o);
   p.lse = a.lse;
-  p.hq = a.hq; p.group = a.hq / a.hkv; p.dim = a.dim;
   p.c = a.scale * kLog2e;
   p.err = a.err;
   CUtensorMap mq, mk, mv;
