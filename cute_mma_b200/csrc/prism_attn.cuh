@@ -100,14 +100,22 @@ __device__ __forceinline__ void attn_zero_gap(const AttnRows& r, const AttnWork&
   }
 }
 
-// A bounded wait by a whole warp, which stays together: false for all lanes if it ran out for one.
+// A bounded wait by a whole warp, which stays together: false for all lanes if it ran out for one.  (One test and a vote
+// where the phase is over already, which is what the issuing warps mostly meet.)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, clock64() - t0 > PRISM_WAIT_LIMIT_CYCLES)) return false;
+  }
 }
 
 // The work of a CTA: it begins with the tile of its own block index and then takes over blocks that have not started yet
 // (cluster launch control), so that the loads and first products of the next tile run beside the end of this one and no
-// CTA is set up twice.  One warp of the CTA looks for work ahead and hands it to the others through two slots.
+// CTA is set up twice.  The warp that loads looks for work ahead and hands it to the others through two slots.
 struct AttnSched {
   uint64_t full[2], empty[2], answer_full;
   alignas(16) uint64_t answer[2];
@@ -145,14 +153,17 @@ __device__ __forceinline__ int clc_answer(const uint64_t* answer) {
   return took ? (int)x : -1;
 }
 
-// The warp that looks for work.  zero(work, head): what to do for a tile that there is none of.
-template <typename Zero>
-__device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows, int heads, int bm, bool last_first, Zero zero) {
+// The warp that looks for work and brings its tiles in.  load(work, head) returns false if a wait ran out; zero(work, head):
+// what to do for a tile that there is none of.
+template <typename Load, typename Zero>
+__device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows, int heads, int bm, bool last_first, Load load,
+                                              Zero zero) {
   const int lane = threadIdx.x & 31;
   Ring r(2);
   uint32_t phase = 0;
   int idx = blockIdx.x;
-  while (idx >= 0) {
+  bool ok = true;
+  while (ok && idx >= 0) {
     if (lane == 0) {
       mbar_arrive_expect_tx(&s.answer_full, 16);
       clc_try_cancel(s.answer, &s.answer_full);
@@ -162,24 +173,23 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
     if (w.tile < 0) {
       zero(w, head);
     } else {
-      if (!warp_wait(&s.empty[r.idx], r.phase ^ 1)) {
-        warp_wait(&s.answer_full, phase);   // its answer is still on the way into this CTA's memory
-        return false;
-      }
-      if (lane == 0) {
+      ok = warp_wait(&s.empty[r.idx], r.phase ^ 1);
+      if (ok && lane == 0) {
         s.work[r.idx] = w;
         s.head[r.idx] = head;
         mbar_arrive(&s.full[r.idx]);
       }
       r.next();
+      ok = ok && load(w, head);
     }
-    if (!warp_wait(&s.answer_full, phase)) return false;
+    // (the answer is waited for in any case: it is on its way into this CTA's memory)
+    if (!warp_wait(&s.answer_full, phase)) ok = false;
     phase ^= 1u;
-    idx = clc_answer(s.answer);
+    idx = __shfl_sync(0xffffffffu, clc_answer(s.answer), 0);
     fence_proxy_async_smem();   // the answer is read before the next one may overwrite it
     __syncwarp();
   }
-  if (!warp_wait(&s.empty[r.idx], r.phase ^ 1)) return false;
+  if (!ok || !warp_wait(&s.empty[r.idx], r.phase ^ 1)) return false;
   if (lane == 0) {
     s.work[r.idx].tile = -1;
     mbar_arrive(&s.full[r.idx]);
@@ -189,8 +199,14 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
 // The next piece of work for one of the other warps: false at the end (or if the wait ran out, with ok false).
 __device__ __forceinline__ bool attn_next(AttnSched& s, Ring& r, AttnWork* w, int* head, bool* ok) {
   if (!warp_wait(&s.full[r.idx], r.phase)) { *ok = false; return false; }
-  *w = s.work[r.idx];
-  *head = s.head[r.idx];
+  // (through shuffles: the compiler then knows that all lanes have the same)
+  const AttnWork& o = s.work[r.idx];
+  w->tile = __shfl_sync(0xffffffffu, o.tile, 0);
+  w->len = __shfl_sync(0xffffffffu, o.len, 0);
+  w->row = __shfl_sync(0xffffffffu, o.row, 0);
+  w->batch = __shfl_sync(0xffffffffu, o.batch, 0);
+  w->orow = __shfl_sync(0xffffffffu, o.orow, 0);
+  *head = __shfl_sync(0xffffffffu, s.head[r.idx], 0);
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(&s.empty[r.idx]);
   r.next();

@@ -21,8 +21,8 @@ struct BwdParams {
   int* err;
 };
 
-// Two warpgroups of arithmetic, then the MMA warp, the TMA warp, the warp of the row statistics and the one that looks for
-// work.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is launched with.
+// Two warpgroups of arithmetic, and one of the loading warp, the issuing warps and (dk, dv) the warp of the row statistics.
+//  256 x 208 + 128 x 88 registers = 384 x 168, what the block is launched with.
 constexpr int kThreads = 384, kMathRegs = 208, kOtherRegs = 88;
 
 // Every PRISM_ATTN_BWD_POLY-th second pair of exponentials goes to the FMA pipe.
@@ -73,11 +73,11 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const DeltaParams p) {
 template <int DH>
 struct DkvSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
-  static constexpr int kQ = DH == 128 ? 3 : 4, kDo = DH == 128 ? 2 : 4;   // rings of Q and of dO tiles
+  static constexpr int kQ = DH == 128 ? 2 : 4, kDo = DH == 128 ? 3 : 4;   // rings of Q and of dO tiles
   static constexpr uint32_t kBytes = (2 + kQ + kDo) * kTile + 1024;
 };
 struct DkvBars {
-  uint64_t kv_full, kv_empty, s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty;
+  uint64_t kv_full, kv_empty, s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty, clean[2];
   uint64_t q_full[4], q_empty[4], do_full[4], do_empty[4];
 };
 
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 
   if (warp == 8) {
@@ -101,11 +101,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
     attn_sched_init(sched, 11);
+    mbar_init(&bars.clean[0], 1);
+    mbar_init(&bars.clean[1], 1);
     mbar_init(&bars.kv_full, 1);
-    mbar_init(&bars.kv_empty, 1);
+    mbar_init(&bars.kv_empty, 2);
     mbar_init(&bars.dp_full, 1);
     mbar_init(&bars.ds_full, 8);
-    mbar_init(&bars.acc_full, 1);
+    mbar_init(&bars.acc_full, 2);
     mbar_init(&bars.acc_empty, 8);
     mbar_init(&bars.st_full, 1);
     mbar_init(&bars.st_empty, 8);
@@ -117,62 +119,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.q_full[s], 1);
       mbar_init(&bars.q_empty[s], 1);
       mbar_init(&bars.do_full[s], 1);
-      mbar_init(&bars.do_empty[s], 1);
+      mbar_init(&bars.do_empty[s], 2);
     }
     fence_mbar_init();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);   // (known to be the same in all lanes)
   bool ok = true;
   AttnWork w;
   int kvh;
   Ring rw(2);
-  auto q_tiles = [&]() { return (w.len + kAttnTile - 1) / kAttnTile - w.tile; };   // of a head, from the diagonal on
+  auto q_tiles = [](const AttnWork& g) { return (g.len + kAttnTile - 1) / kAttnTile - g.tile; };   // of a head, from the diagonal on
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 11) {
-      ok = attn_schedule(sched, p.rows, p.hkv, kAttnTile, false, [&](const AttnWork& g, int h) {
-        attn_zero_gap(p.rows, g, p.dk, p.hkv, h, p.dim);
-        attn_zero_gap(p.rows, g, p.dv, p.hkv, h, p.dim);
-      });
-    } else if (warp == 9) {
+    if (warp == 9) {
       char *q_ring = smem + 2 * L::kTile, *do_ring = q_ring + L::kQ * L::kTile;
       Ring rq(L::kQ), rd(L::kDo);
       uint32_t used = 0;
-      while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
-        const int nq = q_tiles(), n = nq * p.group;
-        if (!warp_wait(&bars.kv_empty, (used & 1) ^ 1)) { ok = false; break; }
-        ++used;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
-          attn_load_tile<DH>(smem, &mk, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
-          attn_load_tile<DH>(smem + L::kTile, &mv, &bars.kv_full, w.row + w.tile * kAttnTile, kvh, w.batch);
-        }
-        int head = kvh * p.group, i = 0;
-        for (int it = 0; it < n; ++it, rq.next(), rd.next()) {
-          const int row = w.row + (w.tile + i) * kAttnTile;
-          if (!warp_wait(&bars.q_empty[rq.idx], rq.phase ^ 1)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.q_full[rq.idx], L::kTile);
-            attn_load_tile<DH>(q_ring + rq.idx * L::kTile, &mq, &bars.q_full[rq.idx], row, head, w.batch);
-          }
-          if (!warp_wait(&bars.do_empty[rd.idx], rd.phase ^ 1)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.do_full[rd.idx], L::kTile);
-            attn_load_tile<DH>(do_ring + rd.idx * L::kTile, &mdo, &bars.do_full[rd.idx], row, head, w.batch);
-          }
-          if (++i == nq) { i = 0; ++head; }
-        }
-      }
+      ok = attn_schedule(
+          sched, p.rows, p.hkv, kAttnTile, false,
+          [&](const AttnWork& g, int h) {
+            const int nq = q_tiles(g), n = nq * p.group;
+            if (!warp_wait(&bars.kv_empty, (used & 1) ^ 1)) return false;
+            ++used;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
+              attn_load_tile<DH>(smem, &mk, &bars.kv_full, g.row + g.tile * kAttnTile, h, g.batch);
+              attn_load_tile<DH>(smem + L::kTile, &mv, &bars.kv_full, g.row + g.tile * kAttnTile, h, g.batch);
+            }
+            int head = h * p.group, i = 0;
+            for (int it = 0; it < n; ++it, rq.next(), rd.next()) {
+              const int row = g.row + (g.tile + i) * kAttnTile;
+              if (!warp_wait(&bars.q_empty[rq.idx], rq.phase ^ 1)) return false;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.q_full[rq.idx], L::kTile);
+                attn_load_tile<DH>(q_ring + rq.idx * L::kTile, &mq, &bars.q_full[rq.idx], row, head, g.batch);
+              }
+              if (!warp_wait(&bars.do_empty[rd.idx], rd.phase ^ 1)) return false;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.do_full[rd.idx], L::kTile);
+                attn_load_tile<DH>(do_ring + rd.idx * L::kTile, &mdo, &bars.do_full[rd.idx], row, head, g.batch);
+              }
+              if (++i == nq) { i = 0; ++head; }
+            }
+            return true;
+          },
+          [&](const AttnWork& g, int h) {
+            attn_zero_gap(p.rows, g, p.dk, p.hkv, h, p.dim);
+            attn_zero_gap(p.rows, g, p.dv, p.hkv, h, p.dim);
+          });
     } else if (warp == 10) {
-      uint32_t cnt = 0;
+      // the row statistics; and a sequence's last tiles are cleaned behind its end before any product reads them
+      Ring rq(L::kQ), rd(L::kDo);
+      uint32_t cnt = 0, cleaned = 0;
       while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
-        const int nq = q_tiles(), n = nq * p.group;
+        const int nq = q_tiles(w), n = nq * p.group;
         int head = kvh * p.group, i = 0;
-        for (int it = 0; it < n; ++it, ++cnt) {
+        for (int it = 0; it < n; ++it, ++cnt, rq.next(), rd.next()) {
           const long long at = (long long)head * p.rows.rows + w.orow;
           float a[4], b[4];
 #pragma unroll
@@ -180,6 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int row = (w.tile + i) * kAttnTile + e * 32 + lane;
             a[e] = row < w.len ? -__ldg(p.lse + at + row) : -INFINITY;
             b[e] = row < w.len ? -__ldg(p.delta + at + row) : 0.f;
+          }
+          const int valid = w.len - (w.tile + i) * kAttnTile;
+          if (valid < kAttnTile) {
+            if (!warp_wait(&bars.q_full[rq.idx], rq.phase) || !warp_wait(&bars.do_full[rd.idx], rd.phase)) { ok = false; break; }
+            attn_zero_tail<DH>(smem + (2 + rq.idx) * L::kTile, valid);
+            attn_zero_tail<DH>(smem + (2 + L::kQ + rd.idx) * L::kTile, valid);
+            if (lane == 0) mbar_arrive(&bars.clean[cleaned & 1]);   // (two: this warp may be a tile ahead of those that wait)
+            ++cleaned;
           }
           if (!warp_wait(&bars.st_empty, (cnt & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
@@ -192,23 +206,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++i == nq) { i = 0; ++head; }
         }
       }
-    } else if (warp == 8) {
+    } else {
+      // two issuing warps, because a product costs its issuer about as long as the tensor core and every barrier more:
+      // warp 8 has S and dv, whose order on one thread protects S and P in the same columns, warp 11 dP and dk likewise
+      const bool dk_side = warp == 11;
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
       const uint32_t sk = smem_u32(smem), sv = sk + L::kTile, q_ring = sk + 2 * L::kTile, do_ring = q_ring + L::kQ * L::kTile;
       Ring rq(L::kQ), rd(L::kDo);
-      uint32_t used = 0, cnt = 0;   // pieces of work; query tiles of all of them
-      int nq = 0;
-      // the tile is there, and clean behind the sequence
-      auto arrived = [&](uint64_t* full, uint32_t phase, uint32_t offset, int i) {
+      uint32_t used = 0, cnt = 0, cleaned = 0;   // pieces of work; query tiles of all of them, and those that were cleaned
+      // a tile of one of the rings is there, and clean behind the sequence
+      auto arrived = [&](uint64_t* full, uint32_t phase, int i) {
         if (!warp_wait(full, phase)) return false;
-        const int valid = w.len - (w.tile + i) * kAttnTile;
-        if (valid < kAttnTile) attn_zero_tail<DH>(smem + offset, valid);
+        if (w.len - (w.tile + i) * kAttnTile < kAttnTile) {
+          if (!warp_wait(&bars.clean[cleaned & 1], (cleaned >> 1) & 1)) return false;
+          ++cleaned;
+        }
         tc_fence_after_sync();
         return true;
       };
       auto scores = [&](Ring& r, int i, uint32_t c) {
-        if (!arrived(&bars.q_full[r.idx], r.phase, (2 + r.idx) * L::kTile, i)) return false;
-        if (lane == 0) {
+        if (!arrived(&bars.q_full[r.idx], r.phase, i)) return false;
+        if (elect_one()) {
           const uint32_t b = kEarly ? (c & 1) : 0;
           attn_mma_xyt<DH>(tmem + b * 128, sk, q_ring + r.idx * L::kTile, id_s);
           umma_commit_cta(&bars.s_full[b]);
@@ -216,19 +234,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       auto dprobs = [&](Ring& r, int i, bool last) {
-        if (!arrived(&bars.do_full[r.idx], r.phase, (2 + L::kQ + r.idx) * L::kTile, i)) return false;
-        if (lane == 0) {
+        if (!arrived(&bars.do_full[r.idx], r.phase, i)) return false;
+        if (elect_one()) {
           attn_mma_xyt<DH>(tmem + kDp, sv, do_ring + r.idx * L::kTile, id_s);
           umma_commit_cta(&bars.dp_full);
+          umma_commit_cta(&bars.do_empty[r.idx]);
           if (last) umma_commit_cta(&bars.kv_empty);
         }
         return true;
       };
       while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
-        nq = q_tiles();
-        const int n = nq * p.group;
+        const int nq = q_tiles(w), n = nq * p.group;
         int i = 0;
-        ok = warp_wait(&bars.kv_full, used & 1) && scores(rq, 0, cnt) && dprobs(rd, 0, n == 1);
+        ok = warp_wait(&bars.kv_full, used & 1) && (dk_side ? dprobs(rd, 0, n == 1) : scores(rq, 0, cnt));
         for (int it = 0; ok && it < n; ++it, ++cnt) {
           const int valid = w.len - (w.tile + i) * kAttnTile;
           const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
@@ -237,31 +255,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           nrd.next();
           if (++i == nq) i = 0;
           const bool more = it + 1 < n;
-          if (kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
-          const uint32_t dot = do_ring + rd.idx * L::kTile, pt = tmem + (kEarly ? (cnt & 1) * 128 : 0);
-          if (it == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (!warp_wait(&bars.p_full[c], cnt & 1)) { ok = false; break; }
+          if (dk_side) {
+            if (it == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
+            if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
             tc_fence_after_sync();
-            if (lane == 0)
+            if (elect_one()) {
+              attn_mma_py<DH>(tmem + kDk, tmem + kDp, 64, q_ring + rq.idx * L::kTile, id_o, it > 0, steps);
+              umma_commit_cta(&bars.q_empty[rq.idx]);
+              if (!more) umma_commit_cta(&bars.acc_full);
+            }
+            if (more && !dprobs(nrd, i, it + 2 == n)) { ok = false; break; }
+          } else {
+            if (kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
+            const uint32_t dot = do_ring + rd.idx * L::kTile, pt = tmem + (kEarly ? (cnt & 1) * 128 : 0);
+            if (it == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
+            if (!warp_wait(&bars.do_full[rd.idx], rd.phase)) { ok = false; break; }
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if (h * 4 + c * 2 < steps)
-                  attn_mma_py<DH>(tmem + kDv, pt + h * 64 + c * 16, 0, dot + (h * 4 + c * 2) * 2048, id_o,
-                                  it > 0 || c > 0 || h > 0, min(2, steps - h * 4 - c * 2));
+            for (int c = 0; c < 2; ++c) {
+              if (!warp_wait(&bars.p_full[c], cnt & 1)) { ok = false; break; }
+              tc_fence_after_sync();
+              if (elect_one())
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (h * 4 + c * 2 < steps)
+                    attn_mma_py<DH>(tmem + kDv, pt + h * 64 + c * 16, 0, dot + (h * 4 + c * 2) * 2048, id_o,
+                                    it > 0 || c > 0 || h > 0, min(2, steps - h * 4 - c * 2));
+            }
+            if (!ok) break;
+            if (elect_one()) {
+              umma_commit_cta(&bars.do_empty[rd.idx]);
+              if (!more) {
+                umma_commit_cta(&bars.kv_empty);
+                umma_commit_cta(&bars.acc_full);
+              }
+            }
+            if (!kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
           }
-          if (!ok) break;
-          if (lane == 0) umma_commit_cta(&bars.do_empty[rd.idx]);
-          if (!kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
-          if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
-          tc_fence_after_sync();
-          if (lane == 0) {
-            attn_mma_py<DH>(tmem + kDk, tmem + kDp, 64, q_ring + rq.idx * L::kTile, id_o, it > 0, steps);
-            umma_commit_cta(&bars.q_empty[rq.idx]);
-            if (!more) umma_commit_cta(&bars.acc_full);
-          }
-          if (more && !dprobs(nrd, i, it + 2 == n)) { ok = false; break; }
           rq = nrq;
           rd = nrd;
         }
@@ -279,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float4* del = reinterpret_cast<const float4*>(st_delta + half * 64);
     uint32_t cnt = 0, used = 0;
     while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
-      const int nq = q_tiles(), n = nq * p.group;
+      const int nq = q_tiles(w), n = nq * p.group;
       int i = 0;
       for (int it = 0; it < n; ++it, ++cnt) {
         const bool diag = i == 0;
@@ -387,7 +416,7 @@ struct DqSmem {
   static constexpr uint32_t kBytes = (2 + kK + kV) * kTile + 1024;
 };
 struct DqBars {
-  uint64_t q_full, q_empty, s_full, s_read, dp_full[2], ds_full, acc_full, acc_empty;
+  uint64_t q_full, q_empty, s_full, s_read, dp_full[2], ds_full, ds_empty[2], acc_full, acc_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
@@ -401,16 +430,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DqBars bars;
   __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 
   if (warp == 8) {
     tmem_alloc_cta(&tmem_slot, 512);
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
-    attn_sched_init(sched, 10);
+    attn_sched_init(sched, 11);
     mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 1);
+    mbar_init(&bars.q_empty, 2);
+    mbar_init(&bars.ds_empty[0], 1);
+    mbar_init(&bars.ds_empty[1], 1);
     mbar_init(&bars.s_full, 1);
     mbar_init(&bars.s_read, 8);
     mbar_init(&bars.ds_full, 8);
@@ -429,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);   // (known to be the same in all lanes)
   bool ok = true;
   AttnWork w;
   int head;
@@ -437,83 +468,91 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 11) {
-      ok = attn_schedule(sched, p.rows, p.hq, kAttnTile, true,
-                         [&](const AttnWork& g, int h) { attn_zero_gap(p.rows, g, p.dq, p.hq, h, p.dim); });
-    } else if (warp == 9) {
-      char *k_ring = smem + 2 * L::kTile, *v_ring = k_ring + L::kK * L::kTile;
+    const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
+    const uint32_t sq = smem_u32(smem), sdo = sq + L::kTile, k_ring = sq + 2 * L::kTile, v_ring = k_ring + L::kK * L::kTile;
+    uint32_t used = 0, cnt = 0;   // pieces of work, key tiles of all of them
+    if (warp == 9) {
       Ring rk(L::kK), rv(L::kV);
-      uint32_t used = 0;
+      ok = attn_schedule(
+          sched, p.rows, p.hq, kAttnTile, true,
+          [&](const AttnWork& g, int h) {
+            const int kvh = h / p.group;
+            if (!warp_wait(&bars.q_empty, (used & 1) ^ 1)) return false;
+            ++used;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
+              attn_load_tile<DH>(smem, &mq, &bars.q_full, g.row + g.tile * kAttnTile, h, g.batch);
+              attn_load_tile<DH>(smem + L::kTile, &mdo, &bars.q_full, g.row + g.tile * kAttnTile, h, g.batch);
+            }
+            for (int j = 0; j <= g.tile; ++j, rk.next(), rv.next()) {
+              if (!warp_wait(&bars.k_empty[rk.idx], rk.phase ^ 1)) return false;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.k_full[rk.idx], L::kTile);
+                attn_load_tile<DH>(smem + (2 + rk.idx) * L::kTile, &mk, &bars.k_full[rk.idx], g.row + j * kAttnTile, kvh, g.batch);
+              }
+              if (!warp_wait(&bars.v_empty[rv.idx], rv.phase ^ 1)) return false;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.v_full[rv.idx], L::kTile);
+                attn_load_tile<DH>(smem + (2 + L::kK + rv.idx) * L::kTile, &mv, &bars.v_full[rv.idx], g.row + j * kAttnTile,
+                                   kvh, g.batch);
+              }
+            }
+            return true;
+          },
+          [&](const AttnWork& g, int h) { attn_zero_gap(p.rows, g, p.dq, p.hq, h, p.dim); });
+    } else if (warp == 8) {   // S (three issuing warps: a product costs its issuer about as long as the tensor core)
+      Ring r(L::kK);
       while (ok && attn_next(sched, rw, &w, &head, &ok)) {
-        const int kvh = head / p.group;
-        if (!warp_wait(&bars.q_empty, (used & 1) ^ 1)) { ok = false; break; }
+        ok = warp_wait(&bars.q_full, used & 1);
         ++used;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
-          attn_load_tile<DH>(smem, &mq, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
-          attn_load_tile<DH>(smem + L::kTile, &mdo, &bars.q_full, w.row + w.tile * kAttnTile, head, w.batch);
-        }
-        for (int j = 0; j <= w.tile; ++j, rk.next(), rv.next()) {
-          if (!warp_wait(&bars.k_empty[rk.idx], rk.phase ^ 1)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.k_full[rk.idx], L::kTile);
-            attn_load_tile<DH>(k_ring + rk.idx * L::kTile, &mk, &bars.k_full[rk.idx], w.row + j * kAttnTile, kvh, w.batch);
-          }
-          if (!warp_wait(&bars.v_empty[rv.idx], rv.phase ^ 1)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.v_full[rv.idx], L::kTile);
-            attn_load_tile<DH>(v_ring + rv.idx * L::kTile, &mv, &bars.v_full[rv.idx], w.row + j * kAttnTile, kvh, w.batch);
+        for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
+          if (!warp_wait(&bars.k_full[r.idx], r.phase)) { ok = false; break; }
+          const int valid = w.len - j * kAttnTile;
+          if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + r.idx) * L::kTile, valid);   // for dq's product
+          if (!warp_wait(&bars.s_read, (cnt & 1) ^ 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            attn_mma_xyt<DH>(tmem, sq, k_ring + r.idx * L::kTile, id_s);
+            umma_commit_cta(&bars.s_full);
+            if (j == w.tile) umma_commit_cta(&bars.q_empty);
           }
         }
       }
-    } else if (warp == 8) {
-      const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t sq = smem_u32(smem), sdo = sq + L::kTile, k_ring = sq + 2 * L::kTile, v_ring = k_ring + L::kK * L::kTile;
-      Ring rk(L::kK), rs(L::kK), rv(L::kV);   // key tiles of dq and of the scores (one ahead), value tiles
-      uint32_t used = 0, cnt = 0;
-      auto scores = [&](int j, uint32_t c) {
-        if (!warp_wait(&bars.k_full[rs.idx], rs.phase) || !warp_wait(&bars.s_read, (c & 1) ^ 1)) return false;
-        const int valid = w.len - j * kAttnTile;
-        if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rs.idx) * L::kTile, valid);
-        tc_fence_after_sync();
-        if (lane == 0) {
-          attn_mma_xyt<DH>(tmem, sq, k_ring + rs.idx * L::kTile, id_s);
-          umma_commit_cta(&bars.s_full);
-        }
-        rs.next();
-        return true;
-      };
-      auto dprobs = [&](uint32_t c, bool last) {
-        if (!warp_wait(&bars.v_full[rv.idx], rv.phase)) return false;
-        tc_fence_after_sync();
-        if (lane == 0) {
-          attn_mma_xyt<DH>(tmem + kDp + (c & 1) * 128, sdo, v_ring + rv.idx * L::kTile, id_s);
-          umma_commit_cta(&bars.dp_full[c & 1]);
-          umma_commit_cta(&bars.v_empty[rv.idx]);
-          if (last) umma_commit_cta(&bars.q_empty);
-        }
-        rv.next();
-        return true;
-      };
+    } else if (warp == 10) {   // dP
+      Ring r(L::kV);
       while (ok && attn_next(sched, rw, &w, &head, &ok)) {
-        const int n = w.tile + 1;   // key tiles up to the diagonal
-        ok = warp_wait(&bars.q_full, used & 1) && scores(0, cnt) && dprobs(cnt, n == 1);
-        for (int j = 0; ok && j < n; ++j, ++cnt) {
-          const bool more = j + 1 < n;
-          if (more && !(scores(j + 1, cnt + 1) && dprobs(cnt + 1, j + 2 == n))) { ok = false; break; }
-          if (j == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
+        ok = warp_wait(&bars.q_full, used & 1);
+        ++used;
+        for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
+          if (!warp_wait(&bars.v_full[r.idx], r.phase)) { ok = false; break; }
+          // dS of two tiles ago, in the same columns, has gone into dq
+          if (!warp_wait(&bars.ds_empty[cnt & 1], ((cnt >> 1) & 1) ^ 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            attn_mma_xyt<DH>(tmem + kDp + (cnt & 1) * 128, sdo, v_ring + r.idx * L::kTile, id_s);
+            umma_commit_cta(&bars.dp_full[cnt & 1]);
+            umma_commit_cta(&bars.v_empty[r.idx]);
+            if (j == w.tile) umma_commit_cta(&bars.q_empty);
+          }
+        }
+      }
+    } else {   // dq
+      Ring r(L::kK);
+      while (ok && attn_next(sched, rw, &w, &head, &ok)) {
+        ok = warp_wait(&bars.acc_empty, (used & 1) ^ 1);
+        ++used;
+        for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
           if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
           tc_fence_after_sync();
           const int valid = w.len - j * kAttnTile;
-          if (lane == 0) {
-            attn_mma_py<DH>(tmem + kDq, tmem + kDp + (cnt & 1) * 128, 64, k_ring + rk.idx * L::kTile, id_o, j > 0,
+          if (elect_one()) {
+            attn_mma_py<DH>(tmem + kDq, tmem + kDp + (cnt & 1) * 128, 64, k_ring + r.idx * L::kTile, id_o, j > 0,
                             valid >= kAttnTile ? 8 : (valid + 15) >> 4);
-            umma_commit_cta(&bars.k_empty[rk.idx]);
-            if (!more) umma_commit_cta(&bars.acc_full);
+            umma_commit_cta(&bars.k_empty[r.idx]);
+            umma_commit_cta(&bars.ds_empty[cnt & 1]);
+            if (j == w.tile) umma_commit_cta(&bars.acc_full);
           }
-          rk.next();
         }
-        ++used;
       }
     }
   } else {

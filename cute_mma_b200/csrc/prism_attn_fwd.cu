@@ -26,8 +26,8 @@ struct FwdParams {
   int* err;
 };
 
-// Two softmax warpgroups, and one of the MMA warp, the TMA warp, the warp that looks for work and one that only lends its
-// registers: a softmax thread holds a row of 128 scores.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is
+// Two softmax warpgroups, and one of the two issuing warps, the loading warp and one that only lends its registers: a
+// softmax thread holds a row of 128 scores.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is
 // launched with.
 constexpr int kThreads = 384, kSoftmaxRegs = 208, kOtherRegs = 88;
 
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ FwdBars bars;
   __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 
   if (warp == 8) {
@@ -100,14 +100,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < L::kRing; ++s) {
       mbar_init(&bars.kv_full[s], 1);
-      mbar_init(&bars.kv_empty[s], 1);
+      mbar_init(&bars.kv_empty[s], 2);
     }
     fence_mbar_init();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);   // (known to be the same in all lanes)
   bool ok = true;
   AttnWork w;
   int slot_head;
@@ -115,114 +115,107 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 11) {
-      ok = attn_schedule(sched, p.rows, p.pair ? p.hq / 2 : p.hq, p.pair ? kAttnTile : 2 * kAttnTile, true,
-                         [&](const AttnWork& g, int h) {
-                           for (int t = 0; t <= p.pair; ++t) attn_zero_gap(p.rows, g, p.o, p.hq, p.pair ? 2 * h + t : h, p.dim);
-                         });
-    } else if (warp == 9) {
+    if (warp == 9) {
       char* ring = smem + 2 * L::kTile;
       Ring r(L::kRing);
       uint32_t used[2] = {0, 0};   // pieces of work that tile t had a part in
-      while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
-        const FwdTiles tl(p, w, slot_head);
-        for (int t = 0; t < 2; ++t) {
-          if (tl.n[t] == 0) continue;
-          if (!warp_wait(&bars.q_empty[t], (used[t] & 1) ^ 1)) { ok = false; break; }
-          ++used[t];
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.q_full[t], L::kTile);
-            attn_load_tile<DH>(smem + t * L::kTile, &mq, &bars.q_full[t], w.row + tl.row[t], tl.head[t], w.batch);
-          }
-        }
-        const int n = tl.most(), kvh = tl.head[0] / p.group;
-        for (int i = 0; ok && i < 2 * n; ++i, r.next()) {
-          if (!warp_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars.kv_full[r.idx], L::kTile);
-            attn_load_tile<DH>(ring + r.idx * L::kTile, (i & 1) ? &mv : &mk, &bars.kv_full[r.idx],
-                               w.row + (i >> 1) * kAttnTile, kvh, w.batch);
-          }
-        }
-      }
-    } else if (warp == 8) {
+      ok = attn_schedule(
+          sched, p.rows, p.pair ? p.hq / 2 : p.hq, p.pair ? kAttnTile : 2 * kAttnTile, true,
+          [&](const AttnWork& g, int h) {
+            const FwdTiles tl(p, g, h);
+            for (int t = 0; t < 2; ++t) {
+              if (tl.n[t] == 0) continue;
+              if (!warp_wait(&bars.q_empty[t], (used[t] & 1) ^ 1)) return false;
+              ++used[t];
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.q_full[t], L::kTile);
+                attn_load_tile<DH>(smem + t * L::kTile, &mq, &bars.q_full[t], g.row + tl.row[t], tl.head[t], g.batch);
+              }
+            }
+            const int n = tl.most(), kvh = tl.head[0] / p.group;
+            for (int i = 0; i < 2 * n; ++i, r.next()) {
+              if (!warp_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) return false;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.kv_full[r.idx], L::kTile);
+                attn_load_tile<DH>(ring + r.idx * L::kTile, (i & 1) ? &mv : &mk, &bars.kv_full[r.idx],
+                                   g.row + (i >> 1) * kAttnTile, kvh, g.batch);
+              }
+            }
+            return true;
+          },
+          [&](const AttnWork& g, int h) {
+            for (int t = 0; t <= p.pair; ++t) attn_zero_gap(p.rows, g, p.o, p.hq, p.pair ? 2 * h + t : h, p.dim);
+          });
+    } else if (warp == 8 || warp == 10) {
+      // one issuing warp per tile: a product costs its issuer about as long as the tensor core, every barrier more
+      const int t = warp == 10;
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t ring = smem_u32(smem) + 2 * L::kTile;
+      const uint32_t q_tile = smem_u32(smem) + t * L::kTile, ring = smem_u32(smem) + 2 * L::kTile;
+      const uint32_t st = tmem + t * 128, ot = tmem + kO + t * DH, pt = kEarly ? tmem + 256 + t * 64 : st;
       Ring rk(L::kRing);
-      uint32_t used[2] = {0, 0}, made[2] = {0, 0}, blocks[2] = {0, 0};   // work, scores and key blocks of tile t so far
-      // every lane waits (the warp stays together for the zeros of a last tile), one issues
-      auto scores = [&](int t, uint32_t k_tile, bool last) {
+      uint32_t used = 0, made = 0, blocks = 0;   // pieces of work, scores and key blocks so far
+      auto scores = [&](bool last) {
         tc_fence_after_sync();
-        if (lane == 0) {
-          attn_mma_xyt<DH>(tmem + t * 128, smem_u32(smem) + t * L::kTile, k_tile, id_s);
+        if (elect_one()) {
+          attn_mma_xyt<DH>(st, q_tile, ring + rk.idx * L::kTile, id_s);
           umma_commit_cta(&bars.s_full[t]);
+          umma_commit_cta(&bars.kv_empty[rk.idx]);
           if (last) umma_commit_cta(&bars.q_empty[t]);
         }
-        ++made[t];
+        ++made;
       };
       while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
         const FwdTiles tl(p, w, slot_head);
-        const int n = tl.most();
-        Ring rv = rk;
-        rv.next();
-        ok = warp_wait(&bars.kv_full[rk.idx], rk.phase);
-        for (int t = 0; ok && t < 2; ++t) {
-          if (tl.n[t] == 0) continue;
-          if (!warp_wait(&bars.q_full[t], used[t] & 1)) { ok = false; break; }
-          // the scores of the work before have been read (where P took their place, its product came after)
-          if (kEarly && !warp_wait(&bars.s_read[t], (made[t] & 1) ^ 1)) { ok = false; break; }
-          scores(t, ring + rk.idx * L::kTile, tl.n[t] == 1);
-        }
-        if (ok && lane == 0) umma_commit_cta(&bars.kv_empty[rk.idx]);
-        rk.next();
-        rk.next();
-        for (int j = 0; ok && j < n; ++j) {
-          const bool more = j + 1 < n;
+        const int n = tl.most(), nt = tl.n[t];
+        // every lane waits (the warp stays together for the zeros of a last tile), one issues
+        for (int j = -1; ok && j < n; ++j) {
+          // scores of block j + 1, where they need not wait for block j's product
+          Ring rv = rk;   // (for j >= 0: stands on K of block j + 1, V of block j before it)
+          if (j >= 0) {
+            if (rv.idx == 0) { rv.idx = L::kRing; rv.phase ^= 1u; }
+            --rv.idx;
+          }
+          const bool more = j + 1 < n, mine = j + 1 < nt;
           if (more && !warp_wait(&bars.kv_full[rk.idx], rk.phase)) { ok = false; break; }
-          if (kEarly && more) {
-            for (int t = 0; t < 2; ++t) {
-              if (j + 1 >= tl.n[t]) continue;
-              if (!warp_wait(&bars.s_read[t], (made[t] & 1) ^ 1)) { ok = false; break; }
-              scores(t, ring + rk.idx * L::kTile, j + 2 == tl.n[t]);
+          if (more && !mine) {
+            if (elect_one()) mbar_arrive(&bars.kv_empty[rk.idx]);
+          } else if (mine && (kEarly || j < 0)) {
+            if (j < 0 && !warp_wait(&bars.q_full[t], used & 1)) { ok = false; break; }
+            if (kEarly && !warp_wait(&bars.s_read[t], (made & 1) ^ 1)) { ok = false; break; }
+            scores(j + 2 == nt);
+          }
+          if (j >= 0) {
+            if (!warp_wait(&bars.kv_full[rv.idx], rv.phase)) { ok = false; break; }
+            if (j >= nt) {
+              if (elect_one()) mbar_arrive(&bars.kv_empty[rv.idx]);
+            } else {
+              const int valid = w.len - j * kAttnTile;
+              const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
+              if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rv.idx) * L::kTile, valid);   // (both warps, the same zeros)
+              const uint32_t v_tile = ring + rv.idx * L::kTile;
+              if (j == 0 && !warp_wait(&bars.o_empty[t], (used & 1) ^ 1)) { ok = false; break; }
+              if (!warp_wait(&bars.p_full[t][0], blocks & 1)) { ok = false; break; }
+              tc_fence_after_sync();
+              if (elect_one()) attn_mma_py<DH>(ot, pt, 32, v_tile, id_o, j > 0, min(steps, 4));
+              if (!warp_wait(&bars.p_full[t][1], blocks & 1)) { ok = false; break; }
+              tc_fence_after_sync();
+              if (elect_one()) {
+                if (steps > 4) attn_mma_py<DH>(ot, pt + 32, 32, v_tile + 4 * 2048, id_o, true, steps - 4);
+                if (j + 1 == nt) umma_commit_cta(&bars.o_full[t]);
+                else if (kEarly) umma_commit_cta(&bars.pv_done[t]);
+                umma_commit_cta(&bars.kv_empty[rv.idx]);
+              }
+              ++blocks;
+              if (!kEarly && mine) scores(j + 2 == nt);
             }
-            if (!ok) break;
-            if (lane == 0) umma_commit_cta(&bars.kv_empty[rk.idx]);
           }
-          if (!warp_wait(&bars.kv_full[rv.idx], rv.phase)) { ok = false; break; }
-          const int valid = w.len - j * kAttnTile;
-          if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rv.idx) * L::kTile, valid);
-          const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
-          const uint32_t v_tile = ring + rv.idx * L::kTile;
-          for (int t = 0; t < 2; ++t) {
-            if (j >= tl.n[t]) continue;
-            const uint32_t pt = kEarly ? tmem + 256 + t * 64 : tmem + t * 128;
-            if (j == 0 && !warp_wait(&bars.o_empty[t], (used[t] & 1) ^ 1)) { ok = false; break; }
-            if (!warp_wait(&bars.p_full[t][0], blocks[t] & 1)) { ok = false; break; }
-            tc_fence_after_sync();
-            if (lane == 0) attn_mma_py<DH>(tmem + kO + t * DH, pt, 32, v_tile, id_o, j > 0, min(steps, 4));
-            if (!warp_wait(&bars.p_full[t][1], blocks[t] & 1)) { ok = false; break; }
-            tc_fence_after_sync();
-            if (lane == 0) {
-              if (steps > 4) attn_mma_py<DH>(tmem + kO + t * DH, pt + 32, 32, v_tile + 4 * 2048, id_o, true, steps - 4);
-              if (j + 1 == tl.n[t]) umma_commit_cta(&bars.o_full[t]);
-              else if (kEarly) umma_commit_cta(&bars.pv_done[t]);
-            }
-            if (!kEarly && j + 1 < tl.n[t]) scores(t, ring + rk.idx * L::kTile, j + 2 == tl.n[t]);
-            ++blocks[t];
-          }
-          if (!ok) break;
-          if (lane == 0) {
-            umma_commit_cta(&bars.kv_empty[rv.idx]);
-            if (!kEarly && more) umma_commit_cta(&bars.kv_empty[rk.idx]);
-          }
+          // on to the next K: behind V(j + 1), or at the end to the next work's first
           if (more) {
             rk.next();
             rk.next();
           }
-          rv.next();
-          rv.next();
         }
-        for (int t = 0; t < 2; ++t) used[t] += tl.n[t] > 0;
+        used += nt > 0;
       }
     }
   } else {
