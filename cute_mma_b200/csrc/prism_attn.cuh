@@ -33,16 +33,49 @@ struct AttnWork {
 
 __device__ __forceinline__ int attn_clamp(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// The idx-th tile of `bm` rows, by one whole warp.  last_first: the tiles of a sequence in descending order (a causal
-// row tile costs the more the later it is; CTAs start in order of idx, so that the long ones start first).
-// Packed: offsets are taken into [0, rows] and never run backwards, whatever the tensor holds.
-__device__ __forceinline__ AttnWork attn_find(const AttnRows& r, int idx, int bm, bool last_first) {
+// The idx-th tile of `bm` rows, by one whole warp, the costliest first: blocks start in order of idx, and what is long
+// must not start last.  A causal row tile costs the more the later it is (late), a key tile the earlier.  Packed: offsets
+// are taken into [0, rows] and never run backwards, whatever the tensor holds.  Up to 32 kOwn sequences (a lane keeps
+// kOwn tile counts for as long as the CTA lives) are gone through by levels: a sequence of nt tiles has one each of cost
+// 1 to nt, the tiles of cost above L number sum max(0, nt - L), and a binary search finds the level of idx.  More
+// sequences come in their own order (a search by scanning; with so many no single one weighs much).
+constexpr int kOwn = 8;
+struct AttnOrder {
+  int nt[kOwn];
+  int total, most;   // packed, by levels: all tiles, tiles of the longest sequence
+  bool levels;
+};
+__device__ __forceinline__ void attn_range(const AttnRows& r, int b, int* s, int* e) {
+  *s = attn_clamp(__ldg(r.cu + b), 0, r.rows);
+  *e = attn_clamp(__ldg(r.cu + b + 1), *s, r.rows);
+}
+__device__ __forceinline__ AttnOrder attn_order(const AttnRows& r, int bm) {
+  AttnOrder o;
+  o.levels = r.cu != nullptr && r.n <= 32 * kOwn;
+  int sum = 0, top = 0;
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    const int b = k * 32 + (threadIdx.x & 31);
+    o.nt[k] = 0;
+    if (o.levels && b < r.n) {
+      int s, e;
+      attn_range(r, b, &s, &e);
+      o.nt[k] = (e - s + bm - 1) / bm;
+    }
+    sum += o.nt[k];
+    top = max(top, o.nt[k]);
+  }
+  o.total = __reduce_add_sync(0xffffffffu, sum);
+  o.most = __reduce_max_sync(0xffffffffu, top);
+  return o;
+}
+__device__ __forceinline__ AttnWork attn_find(const AttnRows& r, const AttnOrder& o, int idx, int bm, bool late) {
   AttnWork w;
   w.spare = w.n_spare = 0;
   if (r.cu == nullptr) {
     const int nt = (r.len + bm - 1) / bm;
     const int t = idx / r.n;
-    w.tile = last_first ? nt - 1 - t : t;
+    w.tile = late ? nt - 1 - t : t;
     w.len = r.len;
     w.row = 0;
     w.batch = idx - t * r.n;
@@ -50,39 +83,70 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, int idx, int bm
     return w;
   }
   const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int b0 = 0; b0 < r.n; b0 += 32) {
-    const int b = b0 + lane;
-    int s = 0, e = 0;
-    if (b < r.n) {
-      s = attn_clamp(__ldg(r.cu + b), 0, r.rows);
-      e = attn_clamp(__ldg(r.cu + b + 1), s, r.rows);
-    }
-    const int nt = (e - s + bm - 1) / bm;
-    int incl = nt;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += o;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, idx < base + incl);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      const int t = idx - base - (incl - nt);
-      w.tile = __shfl_sync(0xffffffffu, last_first ? nt - 1 - t : t, l);
-      w.len = __shfl_sync(0xffffffffu, e - s, l);
-      w.row = __shfl_sync(0xffffffffu, s, l);
-      w.batch = 0;
-      w.orow = w.row;
-      return w;
-    }
-    base += __shfl_sync(0xffffffffu, incl, 31);
-  }
   w.tile = -1;
   w.len = w.row = w.batch = 0;
-  w.orow = 0;
-  w.spare = idx - base;
-  w.n_spare = r.tiles - base;
+  int base = 0;
+  if (o.levels) {
+    base = o.total;
+    if (idx < o.total) {
+      auto above = [&](int level) {
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < kOwn; ++k) c += max(0, o.nt[k] - level);
+        return (int)__reduce_add_sync(0xffffffffu, c);
+      };
+      int lo = 1, hi = o.most;   // the largest level whose tiles and those above it reach past idx
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (above(mid - 1) > idx) lo = mid;
+        else hi = mid - 1;
+      }
+      int left = idx - above(lo);
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        const unsigned has = __ballot_sync(0xffffffffu, o.nt[k] >= lo);
+        const int c = __popc(has);
+        if (left >= 0 && left < c) {
+          const int l = __fns(has, 0, left + 1);
+          const int nt = __shfl_sync(0xffffffffu, o.nt[k], l);
+          int s, e;
+          attn_range(r, k * 32 + l, &s, &e);
+          w.tile = late ? lo - 1 : nt - lo;
+          w.len = e - s;
+          w.row = s;
+        }
+        left -= c;
+      }
+    }
+  } else {
+    for (int b0 = 0; b0 < r.n; b0 += 32) {
+      const int b = b0 + lane;
+      int s = 0, e = 0;
+      if (b < r.n) attn_range(r, b, &s, &e);
+      const int nt = (e - s + bm - 1) / bm;
+      int incl = nt;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, idx < base + incl);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        const int t = idx - base - (incl - nt);
+        w.tile = __shfl_sync(0xffffffffu, late ? nt - 1 - t : t, l);
+        w.len = __shfl_sync(0xffffffffu, e - s, l);
+        w.row = __shfl_sync(0xffffffffu, s, l);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  w.orow = w.row;
+  if (w.tile < 0) {
+    w.spare = idx - base;
+    w.n_spare = r.tiles - base;
+  }
   return w;
 }
 
@@ -100,15 +164,36 @@ __device__ __forceinline__ void attn_zero_gap(const AttnRows& r, const AttnWork&
   }
 }
 
-// A bounded wait by a whole warp, which stays together: false for all lanes if it ran out for one.  (One test and a vote
-// where the phase is over already, which is what the issuing warps mostly meet.)
+// A bounded wait by a whole warp, which stays together: false for all lanes if it ran out for one.  It polls instead of
+// sleeping in try_wait: the waits of these kernels are links of one chain, and a sleeper wakes some 100 clocks late.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P1;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P1;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+#ifndef PRISM_ATTN_POLL
+#define PRISM_ATTN_POLL 1
+#endif
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+#if PRISM_ATTN_POLL
+#define ATTN_TEST mbar_test
+#else
+#define ATTN_TEST mbar_try_wait
+#endif
+  if (__all_sync(0xffffffffu, ATTN_TEST(bar, parity))) return true;
   const long long t0 = clock64();
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
-      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      if (__all_sync(0xffffffffu, ATTN_TEST(bar, parity))) return true;
     if (__any_sync(0xffffffffu, clock64() - t0 > PRISM_WAIT_LIMIT_CYCLES)) return false;
   }
 }
@@ -156,20 +241,17 @@ __device__ __forceinline__ int clc_answer(const uint64_t* answer) {
 // The warp that looks for work and brings its tiles in.  load(work, head) returns false if a wait ran out; zero(work, head):
 // what to do for a tile that there is none of.
 template <typename Load, typename Zero>
-__device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows, int heads, int bm, bool last_first, Load load,
+__device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows, int heads, int bm, bool late, Load load,
                                               Zero zero) {
   const int lane = threadIdx.x & 31;
   Ring r(2);
   uint32_t phase = 0;
   int idx = blockIdx.x;
   bool ok = true;
+  const AttnOrder order = attn_order(rows, bm);
   while (ok && idx >= 0) {
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&s.answer_full, 16);
-      clc_try_cancel(s.answer, &s.answer_full);
-    }
     const int head = idx % heads;
-    const AttnWork w = attn_find(rows, idx / heads, bm, last_first);
+    const AttnWork w = attn_find(rows, order, idx / heads, bm, late);
     if (w.tile < 0) {
       zero(w, head);
     } else {
@@ -181,6 +263,12 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
       }
       r.next();
       ok = ok && load(w, head);
+    }
+    // the next block is asked for when this one's last tiles are on their way, not before: a CTA with a long one must not
+    // keep a second from the others
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&s.answer_full, 16);
+      clc_try_cancel(s.answer, &s.answer_full);
     }
     // (the answer is waited for in any case: it is on its way into this CTA's memory)
     if (!warp_wait(&s.answer_full, phase)) ok = false;
@@ -240,7 +328,7 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
   const float2 t = add2(x, both(12582912.f));                       // n in the low bits
-  const float2 f = add2(x, mul2(add2(t, both(-12582912.f)), both(-1.f)));
+  const float2 f = fma2(add2(t, both(-12582912.f)), both(-1.f), x);
   float2 p = fma2(f, both(0x1.5bb994p-10f), both(0x1.3cea84p-7f));
   p = fma2(p, f, both(0x1.c6b754p-5f));
   p = fma2(p, f, both(0x1.ebf9bcp-3f));
@@ -262,7 +350,11 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max3_nan(float a, float b, float c) { return max_nan(max_nan(a, b), c); }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Registers -> TMEM: 32 consecutive columns of the thread's own lane.
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {

@@ -73,11 +73,12 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const DeltaParams p) {
 template <int DH>
 struct DkvSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
+  static constexpr int kKv = DH == 128 ? 1 : 2;   // pairs of K and V tiles: the next work's beside this one's
   static constexpr int kQ = DH == 128 ? 2 : 4, kDo = DH == 128 ? 3 : 4;   // rings of Q and of dO tiles
-  static constexpr uint32_t kBytes = (2 + kQ + kDo) * kTile + 1024;
+  static constexpr uint32_t kBytes = (2 * kKv + kQ + kDo) * kTile + 1024;
 };
 struct DkvBars {
-  uint64_t kv_full, kv_empty, s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty, clean[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty, clean[2];
   uint64_t q_full[4], q_empty[4], do_full[4], do_empty[4];
 };
 
@@ -103,8 +104,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_sched_init(sched, 11);
     mbar_init(&bars.clean[0], 1);
     mbar_init(&bars.clean[1], 1);
-    mbar_init(&bars.kv_full, 1);
-    mbar_init(&bars.kv_empty, 2);
     mbar_init(&bars.dp_full, 1);
     mbar_init(&bars.ds_full, 8);
     mbar_init(&bars.acc_full, 2);
@@ -112,6 +111,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.st_full, 1);
     mbar_init(&bars.st_empty, 8);
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.k_full[s], 1);
+      mbar_init(&bars.k_empty[s], 1);
+      mbar_init(&bars.v_full[s], 1);
+      mbar_init(&bars.v_empty[s], 1);
       mbar_init(&bars.s_full[s], 1);
       mbar_init(&bars.p_full[s], 8);
     }
@@ -136,19 +139,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 9) {
-      char *q_ring = smem + 2 * L::kTile, *do_ring = q_ring + L::kQ * L::kTile;
-      Ring rq(L::kQ), rd(L::kDo);
-      uint32_t used = 0;
+      char *q_ring = smem + 2 * L::kKv * L::kTile, *do_ring = q_ring + L::kQ * L::kTile;
+      Ring rq(L::kQ), rd(L::kDo), rkv(L::kKv);
       ok = attn_schedule(
           sched, p.rows, p.hkv, kAttnTile, false,
           [&](const AttnWork& g, int h) {
             const int nq = q_tiles(g), n = nq * p.group;
-            if (!warp_wait(&bars.kv_empty, (used & 1) ^ 1)) return false;
-            ++used;
+            const int krow = g.row + g.tile * kAttnTile;
+            if (!warp_wait(&bars.k_empty[rkv.idx], rkv.phase ^ 1)) return false;
             if (lane == 0) {
-              mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
-              attn_load_tile<DH>(smem, &mk, &bars.kv_full, g.row + g.tile * kAttnTile, h, g.batch);
-              attn_load_tile<DH>(smem + L::kTile, &mv, &bars.kv_full, g.row + g.tile * kAttnTile, h, g.batch);
+              mbar_arrive_expect_tx(&bars.k_full[rkv.idx], L::kTile);
+              attn_load_tile<DH>(smem + 2 * rkv.idx * L::kTile, &mk, &bars.k_full[rkv.idx], krow, h, g.batch);
             }
             int head = h * p.group, i = 0;
             for (int it = 0; it < n; ++it, rq.next(), rd.next()) {
@@ -158,6 +159,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_arrive_expect_tx(&bars.q_full[rq.idx], L::kTile);
                 attn_load_tile<DH>(q_ring + rq.idx * L::kTile, &mq, &bars.q_full[rq.idx], row, head, g.batch);
               }
+              if (it == 0) {   // (V is given back later than K, and wanted later)
+                if (!warp_wait(&bars.v_empty[rkv.idx], rkv.phase ^ 1)) return false;
+                if (lane == 0) {
+                  mbar_arrive_expect_tx(&bars.v_full[rkv.idx], L::kTile);
+                  attn_load_tile<DH>(smem + (2 * rkv.idx + 1) * L::kTile, &mv, &bars.v_full[rkv.idx], krow, h, g.batch);
+                }
+              }
               if (!warp_wait(&bars.do_empty[rd.idx], rd.phase ^ 1)) return false;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&bars.do_full[rd.idx], L::kTile);
@@ -165,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               if (++i == nq) { i = 0; ++head; }
             }
+            rkv.next();
             return true;
           },
           [&](const AttnWork& g, int h) {
@@ -190,8 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int valid = w.len - (w.tile + i) * kAttnTile;
           if (valid < kAttnTile) {
             if (!warp_wait(&bars.q_full[rq.idx], rq.phase) || !warp_wait(&bars.do_full[rd.idx], rd.phase)) { ok = false; break; }
-            attn_zero_tail<DH>(smem + (2 + rq.idx) * L::kTile, valid);
-            attn_zero_tail<DH>(smem + (2 + L::kQ + rd.idx) * L::kTile, valid);
+            attn_zero_tail<DH>(smem + (2 * L::kKv + rq.idx) * L::kTile, valid);
+            attn_zero_tail<DH>(smem + (2 * L::kKv + L::kQ + rd.idx) * L::kTile, valid);
             if (lane == 0) mbar_arrive(&bars.clean[cleaned & 1]);   // (two: this warp may be a tile ahead of those that wait)
             ++cleaned;
           }
@@ -211,8 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // warp 8 has S and dv, whose order on one thread protects S and P in the same columns, warp 11 dP and dk likewise
       const bool dk_side = warp == 11;
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t sk = smem_u32(smem), sv = sk + L::kTile, q_ring = sk + 2 * L::kTile, do_ring = q_ring + L::kQ * L::kTile;
-      Ring rq(L::kQ), rd(L::kDo);
+      const uint32_t kv = smem_u32(smem), q_ring = kv + 2 * L::kKv * L::kTile, do_ring = q_ring + L::kQ * L::kTile;
+      Ring rq(L::kQ), rd(L::kDo), rkv(L::kKv);
       uint32_t used = 0, cnt = 0, cleaned = 0;   // pieces of work; query tiles of all of them, and those that were cleaned
       // a tile of one of the rings is there, and clean behind the sequence
       auto arrived = [&](uint64_t* full, uint32_t phase, int i) {
@@ -224,29 +233,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after_sync();
         return true;
       };
-      auto scores = [&](Ring& r, int i, uint32_t c) {
-        if (!arrived(&bars.q_full[r.idx], r.phase, i)) return false;
+      auto scores = [&](Ring& r, int i, uint32_t c, bool first, bool last) {
+        if ((kEarly || first) && !arrived(&bars.q_full[r.idx], r.phase, i)) return false;
         if (elect_one()) {
           const uint32_t b = kEarly ? (c & 1) : 0;
-          attn_mma_xyt<DH>(tmem + b * 128, sk, q_ring + r.idx * L::kTile, id_s);
+          attn_mma_xyt<DH>(tmem + b * 128, kv + 2 * rkv.idx * L::kTile, q_ring + r.idx * L::kTile, id_s);
           umma_commit_cta(&bars.s_full[b]);
+          if (last) umma_commit_cta(&bars.k_empty[rkv.idx]);
         }
         return true;
       };
       auto dprobs = [&](Ring& r, int i, bool last) {
         if (!arrived(&bars.do_full[r.idx], r.phase, i)) return false;
         if (elect_one()) {
-          attn_mma_xyt<DH>(tmem + kDp, sv, do_ring + r.idx * L::kTile, id_s);
+          attn_mma_xyt<DH>(tmem + kDp, kv + (2 * rkv.idx + 1) * L::kTile, do_ring + r.idx * L::kTile, id_s);
           umma_commit_cta(&bars.dp_full);
           umma_commit_cta(&bars.do_empty[r.idx]);
-          if (last) umma_commit_cta(&bars.kv_empty);
+          if (last) umma_commit_cta(&bars.v_empty[rkv.idx]);
         }
         return true;
       };
       while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
         const int nq = q_tiles(w), n = nq * p.group;
         int i = 0;
-        ok = warp_wait(&bars.kv_full, used & 1) && (dk_side ? dprobs(rd, 0, n == 1) : scores(rq, 0, cnt));
+        ok = dk_side ? warp_wait(&bars.v_full[rkv.idx], rkv.phase) && dprobs(rd, 0, n == 1)
+                     : warp_wait(&bars.k_full[rkv.idx], rkv.phase) && scores(rq, 0, cnt, true, n == 1);
         for (int it = 0; ok && it < n; ++it, ++cnt) {
           const int valid = w.len - (w.tile + i) * kAttnTile;
           const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
@@ -266,12 +277,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (more && !dprobs(nrd, i, it + 2 == n)) { ok = false; break; }
           } else {
-            if (kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
+            if (kEarly && more && !scores(nrq, i, cnt + 1, false, it + 2 == n)) { ok = false; break; }
             const uint32_t dot = do_ring + rd.idx * L::kTile, pt = tmem + (kEarly ? (cnt & 1) * 128 : 0);
             if (it == 0 && !warp_wait(&bars.acc_empty, (used & 1) ^ 1)) { ok = false; break; }
             if (!warp_wait(&bars.do_full[rd.idx], rd.phase)) { ok = false; break; }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+              // (the next scores' operands are looked for while the second piece is on its way)
+              if (c == 1 && !kEarly && more && !arrived(&bars.q_full[nrq.idx], nrq.phase, i)) { ok = false; break; }
               if (!warp_wait(&bars.p_full[c], cnt & 1)) { ok = false; break; }
               tc_fence_after_sync();
               if (elect_one())
@@ -284,16 +297,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (elect_one()) {
               umma_commit_cta(&bars.do_empty[rd.idx]);
-              if (!more) {
-                umma_commit_cta(&bars.kv_empty);
-                umma_commit_cta(&bars.acc_full);
-              }
+              if (!more) umma_commit_cta(&bars.acc_full);
             }
-            if (!kEarly && more && !scores(nrq, i, cnt + 1)) { ok = false; break; }
+            if (!kEarly && more && !scores(nrq, i, cnt + 1, false, it + 2 == n)) { ok = false; break; }
           }
           rq = nrq;
           rd = nrd;
         }
+        rkv.next();
         ++used;
       }
     }
@@ -413,10 +424,11 @@ template <int DH>
 struct DqSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
   static constexpr int kK = DH == 128 ? 3 : 4, kV = DH == 128 ? 2 : 4;   // rings of K and of V tiles
-  static constexpr uint32_t kBytes = (2 + kK + kV) * kTile + 1024;
+  static constexpr int kQ = DH == 128 ? 1 : 2;   // pairs of Q and dO tiles: the next work's beside this one's
+  static constexpr uint32_t kBytes = (2 * kQ + kK + kV) * kTile + 1024;
 };
 struct DqBars {
-  uint64_t q_full, q_empty, s_full, s_read, dp_full[2], ds_full, ds_empty[2], acc_full, acc_empty;
+  uint64_t q_full[2], q_empty[2], do_full[2], do_empty[2], s_full, s_read, dp_full[2], ds_full, ds_empty[2], acc_full, acc_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
@@ -438,8 +450,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
     attn_sched_init(sched, 11);
-    mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 2);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.q_full[s], 1);
+      mbar_init(&bars.q_empty[s], 1);
+      mbar_init(&bars.do_full[s], 1);
+      mbar_init(&bars.do_empty[s], 1);
+    }
     mbar_init(&bars.ds_empty[0], 1);
     mbar_init(&bars.ds_empty[1], 1);
     mbar_init(&bars.s_full, 1);
@@ -469,72 +485,80 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-    const uint32_t sq = smem_u32(smem), sdo = sq + L::kTile, k_ring = sq + 2 * L::kTile, v_ring = k_ring + L::kK * L::kTile;
+    const uint32_t sq = smem_u32(smem), k_ring = sq + 2 * L::kQ * L::kTile, v_ring = k_ring + L::kK * L::kTile;
     uint32_t used = 0, cnt = 0;   // pieces of work, key tiles of all of them
+    Ring rq(L::kQ);
     if (warp == 9) {
       Ring rk(L::kK), rv(L::kV);
       ok = attn_schedule(
           sched, p.rows, p.hq, kAttnTile, true,
           [&](const AttnWork& g, int h) {
             const int kvh = h / p.group;
-            if (!warp_wait(&bars.q_empty, (used & 1) ^ 1)) return false;
-            ++used;
+            const int row = g.row + g.tile * kAttnTile;
+            if (!warp_wait(&bars.q_empty[rq.idx], rq.phase ^ 1)) return false;
             if (lane == 0) {
-              mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
-              attn_load_tile<DH>(smem, &mq, &bars.q_full, g.row + g.tile * kAttnTile, h, g.batch);
-              attn_load_tile<DH>(smem + L::kTile, &mdo, &bars.q_full, g.row + g.tile * kAttnTile, h, g.batch);
+              mbar_arrive_expect_tx(&bars.q_full[rq.idx], L::kTile);
+              attn_load_tile<DH>(smem + 2 * rq.idx * L::kTile, &mq, &bars.q_full[rq.idx], row, h, g.batch);
             }
             for (int j = 0; j <= g.tile; ++j, rk.next(), rv.next()) {
               if (!warp_wait(&bars.k_empty[rk.idx], rk.phase ^ 1)) return false;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&bars.k_full[rk.idx], L::kTile);
-                attn_load_tile<DH>(smem + (2 + rk.idx) * L::kTile, &mk, &bars.k_full[rk.idx], g.row + j * kAttnTile, kvh, g.batch);
+                attn_load_tile<DH>(smem + (2 * L::kQ + rk.idx) * L::kTile, &mk, &bars.k_full[rk.idx], g.row + j * kAttnTile, kvh, g.batch);
+              }
+              if (j == 0) {
+                if (!warp_wait(&bars.do_empty[rq.idx], rq.phase ^ 1)) return false;
+                if (lane == 0) {
+                  mbar_arrive_expect_tx(&bars.do_full[rq.idx], L::kTile);
+                  attn_load_tile<DH>(smem + (2 * rq.idx + 1) * L::kTile, &mdo, &bars.do_full[rq.idx], row, h, g.batch);
+                }
               }
               if (!warp_wait(&bars.v_empty[rv.idx], rv.phase ^ 1)) return false;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&bars.v_full[rv.idx], L::kTile);
-                attn_load_tile<DH>(smem + (2 + L::kK + rv.idx) * L::kTile, &mv, &bars.v_full[rv.idx], g.row + j * kAttnTile,
+                attn_load_tile<DH>(smem + (2 * L::kQ + L::kK + rv.idx) * L::kTile, &mv, &bars.v_full[rv.idx], g.row + j * kAttnTile,
                                    kvh, g.batch);
               }
             }
+            rq.next();
             return true;
           },
           [&](const AttnWork& g, int h) { attn_zero_gap(p.rows, g, p.dq, p.hq, h, p.dim); });
     } else if (warp == 8) {   // S (three issuing warps: a product costs its issuer about as long as the tensor core)
       Ring r(L::kK);
       while (ok && attn_next(sched, rw, &w, &head, &ok)) {
-        ok = warp_wait(&bars.q_full, used & 1);
-        ++used;
+        ok = warp_wait(&bars.q_full[rq.idx], rq.phase);
         for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
           if (!warp_wait(&bars.k_full[r.idx], r.phase)) { ok = false; break; }
           const int valid = w.len - j * kAttnTile;
-          if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + r.idx) * L::kTile, valid);   // for dq's product
+          if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 * L::kQ + r.idx) * L::kTile, valid);   // for dq's product
           if (!warp_wait(&bars.s_read, (cnt & 1) ^ 1)) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
-            attn_mma_xyt<DH>(tmem, sq, k_ring + r.idx * L::kTile, id_s);
+            attn_mma_xyt<DH>(tmem, sq + 2 * rq.idx * L::kTile, k_ring + r.idx * L::kTile, id_s);
             umma_commit_cta(&bars.s_full);
-            if (j == w.tile) umma_commit_cta(&bars.q_empty);
+            if (j == w.tile) umma_commit_cta(&bars.q_empty[rq.idx]);
           }
         }
+        rq.next();
       }
     } else if (warp == 10) {   // dP
       Ring r(L::kV);
       while (ok && attn_next(sched, rw, &w, &head, &ok)) {
-        ok = warp_wait(&bars.q_full, used & 1);
-        ++used;
+        ok = warp_wait(&bars.do_full[rq.idx], rq.phase);
         for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
           if (!warp_wait(&bars.v_full[r.idx], r.phase)) { ok = false; break; }
           // dS of two tiles ago, in the same columns, has gone into dq
           if (!warp_wait(&bars.ds_empty[cnt & 1], ((cnt >> 1) & 1) ^ 1)) { ok = false; break; }
           tc_fence_after_sync();
           if (elect_one()) {
-            attn_mma_xyt<DH>(tmem + kDp + (cnt & 1) * 128, sdo, v_ring + r.idx * L::kTile, id_s);
+            attn_mma_xyt<DH>(tmem + kDp + (cnt & 1) * 128, sq + (2 * rq.idx + 1) * L::kTile, v_ring + r.idx * L::kTile, id_s);
             umma_commit_cta(&bars.dp_full[cnt & 1]);
             umma_commit_cta(&bars.v_empty[r.idx]);
-            if (j == w.tile) umma_commit_cta(&bars.q_empty);
+            if (j == w.tile) umma_commit_cta(&bars.do_empty[rq.idx]);
           }
         }
+        rq.next();
       }
     } else {   // dq
       Ring r(L::kK);

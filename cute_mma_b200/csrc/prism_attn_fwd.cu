@@ -34,12 +34,14 @@ constexpr int kThreads = 384, kSoftmaxRegs = 208, kOtherRegs = 88;
 template <int DH>
 struct FwdSmem {
   static constexpr uint32_t kTile = (DH / 64) * kAttnSub;
-  static constexpr int kRing = DH == 128 ? 5 : 10;
-  static constexpr uint32_t kBytes = (2 + kRing) * kTile + 1024;
+  static constexpr int kQ = DH == 128 ? 1 : 2;   // pairs of Q tiles: the next work's beside this one's
+  static constexpr int kRing = DH == 128 ? 5 : 9;
+  static constexpr uint32_t kBytes = (2 * kQ + kRing) * kTile + 1024;
 };
 
 struct FwdBars {
-  uint64_t q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
+  uint64_t q_full[2][2], q_empty[2][2], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
+  uint64_t turn[2][4];
   uint64_t kv_full[10], kv_empty[10];
 };
 
@@ -65,7 +67,10 @@ struct FwdTiles {
 
 // Every kPolyOf-th pair of exponentials goes to the FMA pipe.
 #ifndef PRISM_ATTN_FWD_POLY
-#define PRISM_ATTN_FWD_POLY 4
+#define PRISM_ATTN_FWD_POLY 1000
+#endif
+#ifndef PRISM_ATTN_FWD_C0
+#define PRISM_ATTN_FWD_C0 64
 #endif
 
 template <int DT, int DH>
@@ -75,6 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = FwdSmem<DH>;
   constexpr bool kEarly = DH == 64;   // S does not share its columns with P
   constexpr uint32_t kO = kEarly ? 384 : 256;
+  constexpr int kFirst = PRISM_ATTN_FWD_C0;   // keys of P's first piece
   extern __shared__ uint8_t smem_raw[];
   __shared__ FwdBars bars;
   __shared__ AttnSched sched;
@@ -88,8 +94,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 9 && lane == 0) {
     attn_sched_init(sched, 10);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars.q_full[t], 1);
-      mbar_init(&bars.q_empty[t], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&bars.turn[t][i], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars.q_full[t][i], 1);
+        mbar_init(&bars.q_empty[t][i], 1);
+      }
       mbar_init(&bars.s_full[t], 1);
       mbar_init(&bars.s_read[t], 4);
       mbar_init(&bars.p_full[t][0], 4);
@@ -116,22 +125,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 9) {
-      char* ring = smem + 2 * L::kTile;
-      Ring r(L::kRing);
-      uint32_t used[2] = {0, 0};   // pieces of work that tile t had a part in
+      char* ring = smem + 2 * L::kQ * L::kTile;
+      Ring r(L::kRing), rq(L::kQ);
       ok = attn_schedule(
           sched, p.rows, p.pair ? p.hq / 2 : p.hq, p.pair ? kAttnTile : 2 * kAttnTile, true,
           [&](const AttnWork& g, int h) {
             const FwdTiles tl(p, g, h);
             for (int t = 0; t < 2; ++t) {
-              if (tl.n[t] == 0) continue;
-              if (!warp_wait(&bars.q_empty[t], (used[t] & 1) ^ 1)) return false;
-              ++used[t];
+              if (!warp_wait(&bars.q_empty[t][rq.idx], rq.phase ^ 1)) return false;
               if (lane == 0) {
-                mbar_arrive_expect_tx(&bars.q_full[t], L::kTile);
-                attn_load_tile<DH>(smem + t * L::kTile, &mq, &bars.q_full[t], g.row + tl.row[t], tl.head[t], g.batch);
+                if (tl.n[t] == 0) {   // no such tile: its warps pass the buffer on
+                  mbar_arrive(&bars.q_full[t][rq.idx]);
+                } else {
+                  mbar_arrive_expect_tx(&bars.q_full[t][rq.idx], L::kTile);
+                  attn_load_tile<DH>(smem + (2 * rq.idx + t) * L::kTile, &mq, &bars.q_full[t][rq.idx], g.row + tl.row[t],
+                                     tl.head[t], g.batch);
+                }
               }
             }
+            rq.next();
             const int n = tl.most(), kvh = tl.head[0] / p.group;
             for (int i = 0; i < 2 * n; ++i, r.next()) {
               if (!warp_wait(&bars.kv_empty[r.idx], r.phase ^ 1)) return false;
@@ -150,23 +162,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       // one issuing warp per tile: a product costs its issuer about as long as the tensor core, every barrier more
       const int t = warp == 10;
       const uint32_t id_s = make_idesc(DT, 128, 128, 0, 0), id_o = make_idesc(DT, 128, DH, 0, 1);
-      const uint32_t q_tile = smem_u32(smem) + t * L::kTile, ring = smem_u32(smem) + 2 * L::kTile;
+      const uint32_t q_tile = smem_u32(smem) + t * L::kTile, ring = smem_u32(smem) + 2 * L::kQ * L::kTile;
       const uint32_t st = tmem + t * 128, ot = tmem + kO + t * DH, pt = kEarly ? tmem + 256 + t * 64 : st;
-      Ring rk(L::kRing);
+      Ring rk(L::kRing), rq(L::kQ);
       uint32_t used = 0, made = 0, blocks = 0;   // pieces of work, scores and key blocks so far
       auto scores = [&](bool last) {
         tc_fence_after_sync();
         if (elect_one()) {
-          attn_mma_xyt<DH>(st, q_tile, ring + rk.idx * L::kTile, id_s);
+          attn_mma_xyt<DH>(st, q_tile + 2 * rq.idx * L::kTile, ring + rk.idx * L::kTile, id_s);
           umma_commit_cta(&bars.s_full[t]);
           umma_commit_cta(&bars.kv_empty[rk.idx]);
-          if (last) umma_commit_cta(&bars.q_empty[t]);
+          if (last) umma_commit_cta(&bars.q_empty[t][rq.idx]);
         }
         ++made;
       };
       while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
         const FwdTiles tl(p, w, slot_head);
         const int n = tl.most(), nt = tl.n[t];
+        ok = warp_wait(&bars.q_full[t][rq.idx], rq.phase);
+        if (ok && nt == 0 && elect_one()) mbar_arrive(&bars.q_empty[t][rq.idx]);
         // every lane waits (the warp stays together for the zeros of a last tile), one issues
         for (int j = -1; ok && j < n; ++j) {
           // scores of block j + 1, where they need not wait for block j's product
@@ -180,7 +194,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (more && !mine) {
             if (elect_one()) mbar_arrive(&bars.kv_empty[rk.idx]);
           } else if (mine && (kEarly || j < 0)) {
-            if (j < 0 && !warp_wait(&bars.q_full[t], used & 1)) { ok = false; break; }
             if (kEarly && !warp_wait(&bars.s_read[t], (made & 1) ^ 1)) { ok = false; break; }
             scores(j + 2 == nt);
           }
@@ -191,16 +204,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               const int valid = w.len - j * kAttnTile;
               const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
-              if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 + rv.idx) * L::kTile, valid);   // (both warps, the same zeros)
+              if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 * L::kQ + rv.idx) * L::kTile, valid);   // (both warps, the same zeros)
               const uint32_t v_tile = ring + rv.idx * L::kTile;
               if (j == 0 && !warp_wait(&bars.o_empty[t], (used & 1) ^ 1)) { ok = false; break; }
               if (!warp_wait(&bars.p_full[t][0], blocks & 1)) { ok = false; break; }
               tc_fence_after_sync();
-              if (elect_one()) attn_mma_py<DH>(ot, pt, 32, v_tile, id_o, j > 0, min(steps, 4));
+              if (elect_one()) attn_mma_py<DH>(ot, pt, 32, v_tile, id_o, j > 0, min(steps, kFirst / 16));
               if (!warp_wait(&bars.p_full[t][1], blocks & 1)) { ok = false; break; }
               tc_fence_after_sync();
               if (elect_one()) {
-                if (steps > 4) attn_mma_py<DH>(ot, pt + 32, 32, v_tile + 4 * 2048, id_o, true, steps - 4);
+                if (steps > kFirst / 16)
+                  attn_mma_py<DH>(ot, pt + kFirst / 2, 32, v_tile + kFirst / 16 * 2048, id_o, true, steps - kFirst / 16);
                 if (j + 1 == nt) umma_commit_cta(&bars.o_full[t]);
                 else if (kEarly) umma_commit_cta(&bars.pv_done[t]);
                 umma_commit_cta(&bars.kv_empty[rv.idx]);
@@ -216,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         used += nt > 0;
+        rq.next();
       }
     }
   } else {
@@ -225,14 +240,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + kO + t * DH;
     const uint32_t p_addr = kEarly ? tmem + lanes + 256 + t * 64 : s_addr;
     const int r = (warp & 3) * 32 + lane;
-    uint32_t phase = 0, used = 0, pv = 0;
+    uint32_t phase = 0, used = 0, pv = 0, turns = 0;
     while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
       const FwdTiles tl(p, w, slot_head);
-      const int nt = tl.n[t];
-      if (nt == 0) continue;
+      const int nt = tl.n[t], n = tl.most();
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < nt; ++j, phase ^= 1u) {
+      for (int j = 0; j < n; ++j) {
+        if (j >= nt) {   // nothing of this tile: the turn passes on
+          if (kEarly) break;
+          if (!warp_wait(&bars.turn[t][warp & 3], (turns & 1) ^ (t ^ 1))) { ok = false; break; }
+          ++turns;
+          if (lane == 0) mbar_arrive(&bars.turn[t ^ 1][warp & 3]);
+          continue;
+        }
         if (!warp_wait(&bars.s_full[t], phase)) { ok = false; break; }
+        phase ^= 1u;
         tc_fence_after_sync();
         uint32_t s[128];
 #pragma unroll
@@ -284,29 +306,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float2 c2 = both(p.c), n2 = both(m == -INFINITY ? 0.f : -m * p.c);
         float2 sum0 = both(0.f), sum1 = both(0.f);
+        // Wide heads: the exponentials of the two warps of a quarter SM take turns, so that one tile's run beside the
+        // other's products (8192 rows, 16 heads of 128: 288 -> 244 us).  Where S does not wait for P V there is nothing to
+        // wait for between them, and turns only cost (heads of 64: 196 -> 216 us).
+        if (!kEarly && !warp_wait(&bars.turn[t][warp & 3], (turns & 1) ^ (t ^ 1))) { ok = false; break; }
+        ++turns;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t* pk = s + h * 32;   // pairs land in the first half of the registers
-#pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const float2 x = fma2(make_float2(__uint_as_float(s[h * 64 + e]), __uint_as_float(s[h * 64 + e + 1])), c2, n2);
-            float2 y;
-            if ((e / 2) % PRISM_ATTN_FWD_POLY == PRISM_ATTN_FWD_POLY - 1) y = ex2_poly2(x);
-            else y = make_float2(ex2(x.x), ex2(x.y));
-            if (e & 2) sum1 = add2(sum1, y);
-            else sum0 = add2(sum0, y);
-            pk[e >> 1] = Elem<DT>::pack(y.x, y.y);
+        for (int e = 0; e < 128; e += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, n2);
+          float2 y;
+          if ((e / 2) % PRISM_ATTN_FWD_POLY == PRISM_ATTN_FWD_POLY - 1) y = ex2_poly2(x);
+          else y = make_float2(ex2(x.x), ex2(x.y));
+          if (e & 2) sum1 = add2(sum1, y);
+          else sum0 = add2(sum0, y);
+          s[e >> 1] = Elem<DT>::pack(y.x, y.y);   // pairs land in the first half of the registers
+          if (e % 32 == 30) tmem_st_x16(p_addr + (e - 30) / 2, s + (e - 30) / 2);
+          if (e + 2 == kFirst || e + 2 == 128) {
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_full[t][e + 2 == 128]);
           }
-          tmem_st_x32(p_addr + h * 32, pk);
-          tmem_st_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.p_full[t][h]);
         }
+        if (!kEarly && lane == 0) mbar_arrive(&bars.turn[t ^ 1][warp & 3]);
         sum0 = add2(sum0, sum1);
         l += sum0.x + sum0.y;
       }
       if (!ok) break;
+      if (nt == 0) continue;
       if (!warp_wait(&bars.o_full[t], used & 1)) { ok = false; break; }
       ++used;
       tc_fence_after_sync();
