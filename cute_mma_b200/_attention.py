@@ -67,30 +67,33 @@ def _check_prompt(q, k, v, cu_seqlens) -> None:
         raise ValueError("cu_seqlens must be a contiguous int32 tensor (sequences + 1,) on the device of q")
 
 
+def _steps(t):
+    """(batch, row, head) strides of a (rows, heads, dim) or (batch, rows, heads, dim) tensor; a single entry has none,
+    and stands as 8."""
+    n, s = t.shape, t.stride()
+    if len(s) == 3:
+        return 8, s[0] if n[0] != 1 else 8, s[1] if n[1] != 1 else 8
+    return s[0] if n[0] != 1 else 8, s[1] if n[1] != 1 else 8, s[2] if n[2] != 1 else 8
+
+
 def _tma_rows(t):
     """t as the kernels can read it: features contiguous, 16-byte steps between rows, heads and batches (a copy where
     that is not so, e.g. of an expanded tensor), and its (batch, row, head) strides."""
-    d = t.shape[-1]
-
-    def steps(x):
-        s = [8 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride()[:-1])]   # a single entry has no stride
-        return s if len(s) == 3 else [8] + s
-
-    s = steps(t)
-    if t.stride(-1) != 1 or any(x <= 0 or x % 8 for x in s) or t.data_ptr() % 16:
+    s = b, r, h = _steps(t)
+    if t.stride(-1) != 1 or b <= 0 or r <= 0 or h <= 0 or (b | r | h) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-        s = steps(t)
+        s = _steps(t)
     return t, s
 
 
 def _attn_forward(q, k, v, cu_seqlens, scale, want_lse):
     """(o, lse or None); q, k, v as checked."""
     hq, d = q.shape[-2:]
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = q.new_empty(q.shape)   # (contiguous; less host time than torch.empty with its keywords)
     rows = q.shape[:-2].numel()
-    lse = torch.empty(hq, rows, dtype=torch.float32, device=q.device) if want_lse else None
+    lse = q.new_empty((hq, rows), dtype=torch.float32) if want_lse else None
     if rows == 0:
         return o, lse
     q, sq = _tma_rows(q)
@@ -117,8 +120,8 @@ def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_d
     """(dq, dk, dv), None for what is not asked for."""
     hq, d = q.shape[-2:]
     rows = q.shape[:-2].numel()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_dq else None
-    dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) if need_dkv else None for _ in range(2))
+    dq = q.new_empty(q.shape) if need_dq else None
+    dk, dv = (k.new_empty(k.shape) if need_dkv else None for _ in range(2))
     if rows == 0 or not (need_dq or need_dkv):
         return dq, dk, dv
     o = o.contiguous()
@@ -128,7 +131,7 @@ def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_d
     v, sv = _tma_rows(v)
     n, length = _sequences(q, cu_seqlens)
     with F._device_scope(q.device):
-        delta = torch.empty(hq, rows, dtype=torch.float32, device=q.device)
+        delta = lse.new_empty(lse.shape)
         ws = F._workspace.get(q.device, 256)
         _lib.check(_lib.lib().prism_attn_bwd(
             d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), F._ptr(dq), F._ptr(dk),
@@ -187,14 +190,20 @@ class _AttentionFn(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
+        # (the decorator costs 14 us of host time, and only a backward that is itself recorded needs it)
+        return (_AttentionFn._recorded if torch.is_grad_enabled() else _AttentionFn._grads)(ctx, d_o)
+
+    @staticmethod
+    def _grads(ctx, d_o):
         q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
         if _plain_eager(d_o, q, k, v, o, lse) and _plain_grad(d_o):
             need = ctx.needs_input_grad
             dq, dk, dv = _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale, need[0], need[1] or need[2])
             return dq, dk if need[1] else None, dv if need[2] else None, None, None
         return *_attention_bwd_op(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale), None, None
+
+    _recorded = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, d_o: _AttentionFn._grads(ctx, d_o)))
 
 
 def causal_attention(q, k, v, cu_seqlens=None, scale=None):
@@ -235,8 +244,8 @@ def _check_decode(q, k, v, lengths) -> None:
         raise ValueError("lengths must be a contiguous int32 tensor (sequences,) on the device of q")
     for name, t in (("k", k), ("v", v)):
         # (a copy of a whole cache per token is not what a caller wants)
-        if t.numel() and (t.stride(-1) != 1 or any(s % 8 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
-                          or t.data_ptr() % 16):
+        x, y, z = _steps(t)
+        if t.numel() and (t.stride(-1) != 1 or (x | y | z) & 7 or t.data_ptr() & 15):
             raise ValueError(f"{name} must have contiguous features, strides that are multiples of 8 elements and start "
                              "on a 16-byte boundary")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -253,20 +262,25 @@ def _(q, k, v, lengths, scale):
     return q.new_empty(q.shape)
 
 
+_scratch_bytes: dict = {}   # (head_dim, device): prism_attn_decode_scratch_bytes there
+
+
 def _decode(q, k, v, lengths, scale):
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = q.new_empty(q.shape)
     b, hq, d = q.shape
     if b == 0:
         return o
-    q, sq = _tma_rows(q)
-    steps = [[0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])] for t in (k, v)]
+    q, (_, sb, sh) = _tma_rows(q)
     L = _lib.lib()
     with F._device_scope(q.device):
-        nbytes = L.prism_attn_decode_scratch_bytes(d)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        key = d, q.device.index
+        nbytes = _scratch_bytes.get(key)
+        if nbytes is None:
+            nbytes = _scratch_bytes[key] = L.prism_attn_decode_scratch_bytes(d)
+        scratch = q.new_empty(nbytes >> 1)
         _lib.check(L.prism_attn_decode(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lengths.data_ptr(), b, k.shape[1], hq, k.shape[2], d,
-            F._DTYPES[q.dtype], scale, _STRIDES8(sq[1], sq[2], *steps[0], *steps[1]), scratch.data_ptr(), nbytes,
+            F._DTYPES[q.dtype], scale, _STRIDES8(sb, sh, *_steps(k), *_steps(v)), scratch.data_ptr(), nbytes,
             F._raw_stream(q.device)))
     return o
 

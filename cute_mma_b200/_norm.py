@@ -54,26 +54,42 @@ def _w_code(weight):
 
 
 def _norm_forward(x, weight, bias, eps, residual, stats):
-    """(y, sum or None, mean, rstd); the statistics only where asked for."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    """(y, sum or None, statistics or None): means and reciprocal standard deviations of the rows as a (2, rows) tensor."""
+    # (new_empty with contiguous strides: less host time than torch.empty with its keywords)
+    y = x.new_empty(x.shape)
+    s = x.new_empty(x.shape) if residual is not None else None
     n = x.shape[-1]
     m = x.numel() // n
-    mean, rstd = (torch.empty(m, dtype=torch.float32, device=x.device) if stats else None for _ in range(2))
+    st = x.new_empty((2, m), dtype=torch.float32) if stats else None
     if m == 0:
-        return y, s, mean, rstd
+        return y, s, st
     x2, ldx = _rows(x)
     r2, ldr = _rows(residual) if residual is not None else (None, 0)
+    mean = st.data_ptr() if stats else None
     with F._device_scope(x.device):
         _lib.check(_lib.lib().prism_layer_norm(
-            x2.data_ptr(), F._ptr(r2), weight.data_ptr(), F._ptr(bias), y.data_ptr(), F._ptr(s), F._ptr(mean), F._ptr(rstd),
-            m, n, F._DTYPES[x.dtype], _w_code(weight), eps, ldx, ldr, F._raw_stream(x.device)))
-    return y, s, mean, rstd
+            x2.data_ptr(), F._ptr(r2), weight.data_ptr(), F._ptr(bias), y.data_ptr(), F._ptr(s), mean,
+            mean + 4 * m if stats else None, m, n, F._DTYPES[x.dtype], _w_code(weight), eps, ldx, ldr, F._raw_stream(x.device)))
+    return y, s, st
 
 
-def _norm_backward(dy, dsum, s, weight, mean, rstd, need_dbias):
+_scratch_cache: dict = {}
+
+
+def _scratch_bytes(L, m, n, device) -> int:
+    """``prism_layer_norm_scratch_bytes`` on the current device, remembered for the latest shapes."""
+    key = (m, n, device.index)
+    nbytes = _scratch_cache.get(key)
+    if nbytes is None:
+        if len(_scratch_cache) >= 512:
+            _scratch_cache.clear()
+        nbytes = _scratch_cache[key] = L.prism_layer_norm_scratch_bytes(m, n)
+    return nbytes
+
+
+def _norm_backward(dy, dsum, s, weight, stats, need_dbias):
     """(dx, dweight, dbias or None) for the rows s that were normalised."""
-    dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    dx = s.new_empty(s.shape)
     dw = torch.empty_like(weight)
     db = torch.empty_like(weight) if need_dbias else None
     n = s.shape[-1]
@@ -85,11 +101,12 @@ def _norm_backward(dy, dsum, s, weight, mean, rstd, need_dbias):
     ds2, ldds = _rows(dsum) if dsum is not None else (None, 0)
     L = _lib.lib()
     with F._device_scope(s.device):
-        nbytes = L.prism_layer_norm_scratch_bytes(m, n)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+        nbytes = _scratch_bytes(L, m, n, s.device)
+        scratch = stats.new_empty(nbytes >> 2)
+        mean = stats.data_ptr()
         _lib.check(L.prism_layer_norm_bwd(
-            dy2.data_ptr(), F._ptr(ds2), s2.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-            dw.data_ptr(), F._ptr(db), m, n, F._DTYPES[s.dtype], _w_code(weight), lddy, ldds, lds, scratch.data_ptr(), nbytes,
+            dy2.data_ptr(), F._ptr(ds2), s2.data_ptr(), weight.data_ptr(), mean, mean + 4 * m, dx.data_ptr(), dw.data_ptr(),
+            F._ptr(db), m, n, F._DTYPES[s.dtype], _w_code(weight), lddy, ldds, lds, scratch.data_ptr(), nbytes,
             F._raw_stream(s.device)))
     return dx, dw, db
 
@@ -99,39 +116,39 @@ def _norm_backward(dy, dsum, s, weight, mean, rstd, need_dbias):
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("prism_b200::layer_norm", mutates_args=())
 def _norm_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, eps: float, residual: torch.Tensor | None
-             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    y, s, mean, rstd = _norm_forward(x, weight, bias, eps, residual, True)
-    return y, x.new_empty(0) if s is None else s, mean, rstd
+             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    y, s, stats = _norm_forward(x, weight, bias, eps, residual, True)
+    return y, x.new_empty(0) if s is None else s, stats
 
 
 @_norm_op.register_fake
 def _(x, weight, bias, eps, residual):
-    stat = x.new_empty(x.shape[:-1].numel(), dtype=torch.float32)
-    return x.new_empty(x.shape), x.new_empty(0 if residual is None else x.shape), stat, torch.empty_like(stat)
+    return (x.new_empty(x.shape), x.new_empty(0 if residual is None else x.shape),
+            x.new_empty((2, x.shape[:-1].numel()), dtype=torch.float32))
 
 
 @torch.library.custom_op("prism_b200::layer_norm_backward", mutates_args=())
-def _norm_bwd_op(dy: torch.Tensor, dsum: torch.Tensor | None, s: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
-                 rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _norm_backward(dy, dsum, s, weight, mean, rstd, True)
+def _norm_bwd_op(dy: torch.Tensor, dsum: torch.Tensor | None, s: torch.Tensor, weight: torch.Tensor, stats: torch.Tensor
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _norm_backward(dy, dsum, s, weight, stats, True)
 
 
 @_norm_bwd_op.register_fake
-def _(dy, dsum, s, weight, mean, rstd):
+def _(dy, dsum, s, weight, stats):
     return s.new_empty(s.shape), torch.empty_like(weight), torch.empty_like(weight)
 
 
 def _norm_setup(ctx, inputs, output):
     x, weight, bias, eps, residual = inputs
-    _, s, mean, rstd = output
-    ctx.save_for_backward(x if residual is None else s, weight, mean, rstd)
+    _, s, stats = output
+    ctx.save_for_backward(x if residual is None else s, weight, stats)
     ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
-    ctx.mark_non_differentiable(mean, rstd, *(() if residual is not None else (s,)))
+    ctx.mark_non_differentiable(stats, *(() if residual is not None else (s,)))
 
 
-def _norm_grad(ctx, dy, dsum, _dmean, _drstd):
-    s, weight, mean, rstd = ctx.saved_tensors
-    dx, dw, db = _norm_bwd_op(dy, dsum if ctx.has_residual else None, s, weight, mean, rstd)
+def _norm_grad(ctx, dy, dsum, _dstats):
+    s, weight, stats = ctx.saved_tensors
+    dx, dw, db = _norm_bwd_op(dy, dsum if ctx.has_residual else None, s, weight, stats)
     return dx, dw, db if ctx.has_bias else None, None, dx.clone() if ctx.has_residual else None
 
 
@@ -141,25 +158,31 @@ _norm_op.register_autograd(_norm_grad, setup_context=_norm_setup)
 class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual):
-        y, s, mean, rstd = _norm_forward(x, weight, bias, eps, residual, True)
-        ctx.save_for_backward(x if residual is None else s, weight, mean, rstd)
+        y, s, stats = _norm_forward(x, weight, bias, eps, residual, True)
+        ctx.save_for_backward(x if residual is None else s, weight, stats)
         ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
         ctx.set_materialize_grads(False)
         return y if residual is None else (y, s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
-        s, weight, mean, rstd = ctx.saved_tensors
+        # (the decorator costs 14 us of host time, and only a backward that is itself recorded needs it)
+        return (_NormFn._recorded if torch.is_grad_enabled() else _NormFn._grads)(ctx, dy, dsum)
+
+    @staticmethod
+    def _grads(ctx, dy, dsum):
+        s, weight, stats = ctx.saved_tensors
         if dy is None:
             # only the sum was used: its gradient is x's and the residual's
             return dsum, None, None, None, dsum
-        plain = _plain_eager(dy, dsum, s, weight, mean, rstd) and _plain_grad(dy) and (dsum is None or _plain_grad(dsum))
+        plain = _plain_eager(dy, dsum, s, weight, stats) and _plain_grad(dy) and (dsum is None or _plain_grad(dsum))
         if plain:
-            dx, dw, db = _norm_backward(dy, dsum, s, weight, mean, rstd, ctx.has_bias)
+            dx, dw, db = _norm_backward(dy, dsum, s, weight, stats, ctx.has_bias)
         else:
-            dx, dw, db = _norm_bwd_op(dy, dsum, s, weight, mean, rstd)
+            dx, dw, db = _norm_bwd_op(dy, dsum, s, weight, stats)
         return dx, dw, db if ctx.has_bias else None, None, dx if ctx.has_residual else None
+
+    _recorded = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, dy, dsum: _NormFn._grads(ctx, dy, dsum)))
 
 
 def layer_norm(x, weight, bias=None, eps: float = 1e-5, residual=None):
@@ -175,9 +198,9 @@ def layer_norm(x, weight, bias=None, eps: float = 1e-5, residual=None):
     if _plain_eager(x, weight, bias, residual):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
             return _NormFn.apply(x, weight, bias, eps, residual)
-        y, s, _, _ = _norm_forward(x, weight, bias, eps, residual, False)
+        y, s, _ = _norm_forward(x, weight, bias, eps, residual, False)
         return y if residual is None else (y, s)
-    y, s, _, _ = _norm_op(x, weight, bias, eps, residual)
+    y, s, _ = _norm_op(x, weight, bias, eps, residual)
     return y if residual is None else (y, s)
 
 

@@ -96,7 +96,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 template <int KD>   // 16-feature steps
 struct DecodeSmem {
-  static constexpr int kPitch = KD * 32 + 16;                 // bytes of a row: an odd number of 16-byte pieces
+  // Rows of 16-byte pieces without bank conflicts for ldmatrix: an odd number of pieces to a row; at the widest, where the
+  // padding would leave room for one CTA to an SM only, the pieces of a row in an order of its own instead.
+  static constexpr bool kSwizzle = KD == 8;
+  static constexpr int kPitch = KD * 32 + (kSwizzle ? 0 : 16);
+  __device__ static __forceinline__ uint32_t at(int row, int piece) {
+    return row * kPitch + ((kSwizzle ? piece ^ (row & 7) : piece) << 4);
+  }
   static constexpr int kSlice = kKeys * kPitch;               // 16 rows of K or of V
   static constexpr int kRing = kStages * 2 * kSlice;          // of one warp
   static constexpr int kJoin = 2 * kHeads * (KD * 16 + 2) * 4;   // two warps' results
@@ -104,7 +110,7 @@ struct DecodeSmem {
 };
 
 template <int DT, int KD>
-__global__ void __launch_bounds__(kWarps * 32, 2) attn_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kWarps * 32, KD <= 4 ? 3 : 2) attn_decode_kernel(const DecodeParams p) {
   using L = DecodeSmem<KD>;
   extern __shared__ __align__(16) uint8_t dsmem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -147,24 +153,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_decode_kernel(const Decod
   Cursor cur = ld;
   const int n = (int)(last - first);
   const uint32_t ring = smem_u32(dsmem) + warp * L::kRing;
-  const int pieces = p.dim >> 3;
+  // a lane copies the same piece of every kPer-th row
+  constexpr int kPer = 32 / (2 * KD), kRounds = (kKeys + kPer - 1) / kPer;
+  const int lr = lane / (2 * KD), piece = lane - lr * 2 * KD;
+  const bool active = lr < kPer, inside = active && piece < (p.dim >> 3);   // (features behind the head: zeros)
+  uint32_t at[kRounds];
+#pragma unroll
+  for (int e = 0; e < kRounds; ++e) at[e] = L::at(min(e * kPer + lr, kKeys - 1), piece);
+  const uint16_t *kp = nullptr, *vp = nullptr;   // this lane's piece of the head's first row
+  bool moved = true;                             // the head has changed
   auto issue = [&](int i) {
     if (i < n) {
       const uint32_t dst = ring + (i % kStages) * 2 * L::kSlice;
-      const int kvh = ld.hc / p.chunks;
-      const uint16_t* k = p.k + ld.b * p.sk.batch + kvh * p.sk.head;
-      const uint16_t* v = p.v + ld.b * p.sv.batch + kvh * p.sv.head;
-      const int row0 = ld.t * kTileKeys + warp * kKeys;
-#pragma unroll
-      for (int e = lane; e < kKeys * KD * 2; e += 32) {
-        const int r = e / (KD * 2), c = e - r * (KD * 2);
-        const bool live = row0 + r < ld.len && c < pieces;   // rows behind the length and features behind the head: zeros
-        const long long row = live ? row0 + r : 0;
-        const int col = live ? c * 8 : 0;
-        cp_async16(dst + r * L::kPitch + c * 16, k + row * p.sk.row + col, live);
-        cp_async16(dst + L::kSlice + r * L::kPitch + c * 16, v + row * p.sv.row + col, live);
+      if (moved) {
+        const int kvh = ld.hc / p.chunks;
+        kp = p.k + ld.b * p.sk.batch + kvh * p.sk.head + (inside ? piece * 8 : 0);
+        vp = p.v + ld.b * p.sv.batch + kvh * p.sv.head + (inside ? piece * 8 : 0);
       }
+      const int row0 = ld.t * kTileKeys + warp * kKeys + lr;
+      const uint16_t *kr = kp + row0 * p.sk.row, *vr = vp + row0 * p.sv.row;
+      const bool whole = ld.t + 1 < ld.nt;
+#pragma unroll
+      for (int e = 0; e < kRounds; ++e) {
+        if (active && e * kPer + lr < kKeys) {
+          const bool live = inside && (whole || row0 + e * kPer < ld.len);   // rows behind the length: zeros, nothing read
+          cp_async16(dst + at[e], live ? kr + e * kPer * p.sk.row : p.k, live);
+          cp_async16(dst + L::kSlice + at[e], live ? vr + e * kPer * p.sv.row : p.v, live);
+        }
+      }
+      const int hc = ld.hc, b = ld.b;
       ld.next(p);
+      moved = hc != ld.hc || b != ld.b;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -201,24 +220,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_decode_kernel(const Decod
     __syncwarp();
     issue(i + kStages - 1);
     const uint32_t kt = ring + (i % kStages) * 2 * L::kSlice, vt = kt + L::kSlice;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float s[2][4] = {}, s1[2][4] = {};   // (two chains each: a product waits for the one before on its accumulator)
     {
-      const uint32_t a = kt + ((lane & 7) + (lane >> 4) * 8) * L::kPitch + ((lane >> 3) & 1) * 16;
+      const int row = (lane & 7) + (lane >> 4) * 8, piece = (lane >> 3) & 1;
 #pragma unroll
       for (int d = 0; d < KD; ++d) {
         uint32_t b[4];
-        ldsm4(a + d * 32, b);
-        mma16816<DT>(s[0], qf[d], b[0], b[1]);
-        mma16816<DT>(s[1], qf[d], b[2], b[3]);
+        ldsm4(kt + L::at(row, d * 2 + piece), b);
+        mma16816<DT>(d & 1 ? s1[0] : s[0], qf[d], b[0], b[1]);
+        mma16816<DT>(d & 1 ? s1[1] : s[1], qf[d], b[2], b[3]);
       }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) s[x][f] += s1[x][f];
     }
-    const int key = cur.t * kTileKeys + warp * kKeys + cq;
+    if (cur.t + 1 == cur.nt) {
+      const int key = cur.t * kTileKeys + warp * kKeys + cq;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int f = 0; f < 4; ++f)
-        if (key + x * 8 + (f & 1) >= cur.len) s[x][f] = -INFINITY;
+        for (int f = 0; f < 4; ++f)
+          if (key + x * 8 + (f & 1) >= cur.len) s[x][f] = -INFINITY;
+    }
     uint32_t pf[4];
+    float f2[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {   // rows r0 and r0 + 8
       float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
@@ -226,26 +252,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_decode_kernel(const Decod
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       mx = fmaxf(mx, m[h]);
       const float base = mx == -INFINITY ? 0.f : mx;
-      const float f = ex2((m[h] - base) * p.c);
+      const float f = f2[h] = ex2((m[h] - base) * p.c);
       m[h] = mx;
       const float neg = -base * p.c;
       const float e0 = ex2(fmaf(s[0][2 * h], p.c, neg)), e1 = ex2(fmaf(s[0][2 * h + 1], p.c, neg));
       const float e2 = ex2(fmaf(s[1][2 * h], p.c, neg)), e3 = ex2(fmaf(s[1][2 * h + 1], p.c, neg));
       l[h] = l[h] * f + ((e0 + e1) + (e2 + e3));
-#pragma unroll
-      for (int d = 0; d < 2 * KD; ++d) {
-        o[d][2 * h] *= f;
-        o[d][2 * h + 1] *= f;
-      }
       pf[h] = Elem<DT>::pack(e0, e1);
       pf[2 + h] = Elem<DT>::pack(e2, e3);
     }
+    if (__any_sync(0xffffffffu, f2[0] != 1.f || f2[1] != 1.f)) {   // (a maximum has grown: rare behind the first keys)
+#pragma unroll
+      for (int d = 0; d < 2 * KD; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          o[d][2 * h] *= f2[h];
+          o[d][2 * h + 1] *= f2[h];
+        }
+    }
     {
-      const uint32_t a = vt + (lane & 15) * L::kPitch + (lane >> 4) * 16;
 #pragma unroll
       for (int d = 0; d < KD; ++d) {
         uint32_t b[4];
-        ldsm4_t(a + d * 32, b);
+        ldsm4_t(vt + L::at(lane & 15, d * 2 + (lane >> 4)), b);
         mma16816<DT>(o[2 * d], pf, b[0], b[1]);
         mma16816<DT>(o[2 * d + 1], pf, b[2], b[3]);
       }
@@ -334,12 +363,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) attn_decode_kernel(const Decod
 }
 
 // Joins the pieces of the heads that more than one CTA worked on, and writes zeros for sequences without keys: a CTA per
-// query head, a warp per quarter of its pieces.
+// query head.  First all pieces' maxima and sums, a thread each, which gives their weights; then the weighted values, a
+// quarter of the pieces to a warp.
+constexpr int kMostPieces = 1024;   // CTAs of a launch at most
 template <int DT, int KD>
 __global__ void __launch_bounds__(128) attn_decode_join_kernel(const DecodeParams p) {
   constexpr int kRow = KD * 16 + 2;
-  __shared__ float acc[4][KD * 16];
-  __shared__ float ml[4][2];
+  __shared__ float acc[4][KD * 16], weight[kMostPieces], part_m[4], part_l[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.hq, head = blockIdx.x - b * p.hq;
   const int kvh = head / p.group, in_group = head - kvh * p.group;
@@ -356,44 +386,49 @@ __global__ void __launch_bounds__(128) attn_decode_join_kernel(const DecodeParam
   total *= hcs;
   const long long share = (total + p.ctas - 1) / p.ctas;
   const long long t0 = before * hcs + (long long)hc * nt, t1 = t0 + nt;
-  const int c0 = (int)(t0 / share), c1 = (int)((t1 - 1) / share);
-  if (c0 == c1) return;
+  const int c0 = (int)(t0 / share), pieces = (int)((t1 - 1) / share) - c0 + 1;
+  if (pieces == 1) return;
+  auto piece = [&](int c) { return p.part + (((long long)(c0 + c) * 2 + (c == 0 ? 1 : 0)) * kHeads + row) * kRow; };
+  float m = -INFINITY;
+  for (int c = threadIdx.x; c < pieces; c += 128) {
+    weight[c] = piece(c)[KD * 16];
+    m = max_nan(m, weight[c]);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (lane == 0) part_m[warp] = m;
+  __syncthreads();
+  m = max_nan(max_nan(part_m[0], part_m[1]), max_nan(part_m[2], part_m[3]));
+  if (m == -INFINITY) m = 0.f;
+  float l = 0.f;
+  for (int c = threadIdx.x; c < pieces; c += 128) {
+    const float f = ex2((weight[c] - m) * p.c);
+    weight[c] = f;
+    l += piece(c)[KD * 16 + 1] * f;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (lane == 0) part_l[warp] = l;
+  __syncthreads();
   constexpr int kPer = (KD * 16 + 31) / 32;
-  float m = -INFINITY, l = 0.f, o[kPer];
+  float o[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    const float* src = p.part + (((long long)c * 2 + (c == c0 ? 1 : 0)) * kHeads + row) * kRow;
-    const float m1 = src[KD * 16], l1 = src[KD * 16 + 1];
-    const float mx = fmaxf(m, m1), base = mx == -INFINITY ? 0.f : mx;
-    const float f0 = ex2((m - base) * p.c), f1 = ex2((m1 - base) * p.c);
-    m = mx;
-    l = l * f0 + l1 * f1;
+#pragma unroll 4
+  for (int c = warp; c < pieces; c += 4) {
+    const float* src = piece(c);
+    const float f = weight[c];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int d = e * 32 + lane;
-      if (d < KD * 16) o[e] = o[e] * f0 + src[d] * f1;
-    }
+    for (int e = 0; e < kPer; ++e)
+      if (e * 32 + lane < KD * 16) o[e] = fmaf(src[e * 32 + lane], f, o[e]);
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e)
     if (e * 32 + lane < KD * 16) acc[warp][e * 32 + lane] = o[e];
-  if (lane == 0) {
-    ml[warp][0] = m;
-    ml[warp][1] = l;
-  }
   __syncthreads();
-  float mx = fmaxf(fmaxf(ml[0][0], ml[1][0]), fmaxf(ml[2][0], ml[3][0]));
-  if (mx == -INFINITY) mx = 0.f;
-  float f[4], sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = ex2((ml[w][0] - mx) * p.c);
-    sum += ml[w][1] * f[w];
-  }
-  const float inv = 1.f / sum;
+  const float inv = 1.f / ((part_l[0] + part_l[1]) + (part_l[2] + part_l[3]));
   for (int d = threadIdx.x; d < p.dim; d += 128) {
-    const float x = acc[0][d] * f[0] + acc[1][d] * f[1] + acc[2][d] * f[2] + acc[3][d] * f[3];
+    const float x = (acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d]);
     dst[d] = (uint16_t)(Elem<DT>::pack(x * inv, 0.f) & 0xffffu);
   }
 }
@@ -433,10 +468,14 @@ int launch_d(const DecodeParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-static int decode_ctas(int num_sms) { return 2 * num_sms; }
+// As many CTAs as are resident together: three to an SM for heads of up to 64, two for wider ones (shared memory).
+static int decode_ctas(int dim, int num_sms) {
+  const int n = (dim <= 64 ? 3 : 2) * num_sms;
+  return n < kMostPieces ? n : kMostPieces;
+}
 
 size_t attn_decode_scratch_bytes(int dim, int num_sms) {
-  return (size_t)2 * decode_ctas(num_sms) * kHeads * ((dim + 15) / 16 * 16 + 2) * sizeof(float);
+  return (size_t)2 * decode_ctas(dim, num_sms) * kHeads * ((dim + 15) / 16 * 16 + 2) * sizeof(float);
 }
 
 int launch_attn_decode(const AttnArgs& a, const int* lengths, float* scratch, int num_sms) {
@@ -452,7 +491,7 @@ int launch_attn_decode(const AttnArgs& a, const int* lengths, float* scratch, in
   p.c = a.scale * kLog2e;
   p.o = static_cast<uint16_t*>(a.o);
   p.part = scratch;
-  p.ctas = decode_ctas(num_sms);
+  p.ctas = decode_ctas(a.dim, num_sms);
   if ((long long)p.n * p.hq > 0x7fffffffll) return fail(PRISM_ERR_UNSUPPORTED, "decode attention: more than 2^31 rows");
   return a.dtype == DT_BF16 ? launch_d<DT_BF16>(p, a.stream) : launch_d<DT_F16>(p, a.stream);
 }
