@@ -88,14 +88,16 @@ def _tma_rows(t):
     return t, s
 
 
-def _attn_forward(q, k, v, cu_seqlens, scale, want_lse):
-    """(o, lse or None); q, k, v as checked."""
+def _attn_forward(q, k, v, cu_seqlens, scale, train):
+    """(o, lse, o_low), the latter two for the backward and None without it: the rows' log-sums, and what rounding o took
+    (the backward needs do . o of every row more exactly than o as rounded gives it).  q, k, v as checked."""
     hq, d = q.shape[-2:]
     o = q.new_empty(q.shape)   # (contiguous; less host time than torch.empty with its keywords)
     rows = q.shape[:-2].numel()
-    lse = q.new_empty((hq, rows), dtype=torch.float32) if want_lse else None
+    lse = q.new_empty((hq, rows), dtype=torch.float32) if train else None
+    low = q.new_empty(q.shape, dtype=torch.uint8) if train else None
     if rows == 0:
-        return o, lse
+        return o, lse, low
     q, sq = _tma_rows(q)
     k, sk = _tma_rows(k)
     v, sv = _tma_rows(v)
@@ -103,10 +105,10 @@ def _attn_forward(q, k, v, cu_seqlens, scale, want_lse):
     with F._device_scope(q.device):
         ws = F._workspace.get(q.device, 256)
         _lib.check(_lib.lib().prism_attn_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), F._ptr(lse), F._ptr(cu_seqlens), n, length, rows,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), F._ptr(lse), F._ptr(low), F._ptr(cu_seqlens), n, length, rows,
             hq, k.shape[-2], d, F._DTYPES[q.dtype], scale, _STRIDES9(*sq, *sk, *sv), ws.data_ptr(), ws.numel(),
             F._raw_stream(q.device)))
-    return o, lse
+    return o, lse, low
 
 
 def _sequences(q, cu_seqlens):
@@ -116,7 +118,7 @@ def _sequences(q, cu_seqlens):
     return (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
 
 
-def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_dkv=True):
+def _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, scale, need_dq=True, need_dkv=True):
     """(dq, dk, dv), None for what is not asked for."""
     hq, d = q.shape[-2:]
     rows = q.shape[:-2].numel()
@@ -134,8 +136,8 @@ def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_d
         delta = lse.new_empty(lse.shape)
         ws = F._workspace.get(q.device, 256)
         _lib.check(_lib.lib().prism_attn_bwd(
-            d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), F._ptr(dq), F._ptr(dk),
-            F._ptr(dv), delta.data_ptr(), F._ptr(cu_seqlens), n, length, rows, hq, k.shape[-2], d, F._DTYPES[q.dtype],
+            d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), F._ptr(low), F._ptr(dq),
+            F._ptr(dk), F._ptr(dv), delta.data_ptr(), F._ptr(cu_seqlens), n, length, rows, hq, k.shape[-2], d, F._DTYPES[q.dtype],
             scale, _STRIDES12(*sq, *sk, *sv, *sdo), ws.data_ptr(), ws.numel(), F._raw_stream(q.device)))
     return dq, dk, dv
 
@@ -145,24 +147,25 @@ def _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale, need_dq=True, need_d
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("prism_b200::causal_attention", mutates_args=())
 def _attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None,
-                  scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+                  scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     return _attn_forward(q, k, v, cu_seqlens, scale, True)
 
 
 @_attention_op.register_fake
 def _(q, k, v, cu_seqlens, scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[-2], q.shape[:-2].numel()), dtype=torch.float32)
+    return (q.new_empty(q.shape), q.new_empty((q.shape[-2], q.shape[:-2].numel()), dtype=torch.float32),
+            q.new_empty(q.shape, dtype=torch.uint8))
 
 
 @torch.library.custom_op("prism_b200::causal_attention_backward", mutates_args=())
 def _attention_bwd_op(d_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
-                      lse: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float
+                      lse: torch.Tensor, low: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float
                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, scale)
+    return _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, scale)
 
 
 @_attention_bwd_op.register_fake
-def _(d_o, q, k, v, o, lse, cu_seqlens, scale):
+def _(d_o, q, k, v, o, lse, low, cu_seqlens, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
@@ -170,12 +173,11 @@ def _attention_setup(ctx, inputs, output):
     q, k, v, cu_seqlens, scale = inputs
     ctx.save_for_backward(q, k, v, *output, cu_seqlens)
     ctx.scale = scale
-    ctx.mark_non_differentiable(output[1])
+    ctx.mark_non_differentiable(*output[1:])
 
 
-def _attention_grad(ctx, d_o, _d_lse):
-    q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
-    return *_attention_bwd_op(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale), None, None
+def _attention_grad(ctx, d_o, _d_lse, _d_low):
+    return *_attention_bwd_op(d_o, *ctx.saved_tensors, ctx.scale), None, None
 
 
 _attention_op.register_autograd(_attention_grad, setup_context=_attention_setup)
@@ -184,8 +186,8 @@ _attention_op.register_autograd(_attention_grad, setup_context=_attention_setup)
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
-        o, lse = _attn_forward(q, k, v, cu_seqlens, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        o, lse, low = _attn_forward(q, k, v, cu_seqlens, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, low, cu_seqlens)
         ctx.scale = scale
         return o
 
@@ -196,12 +198,12 @@ class _AttentionFn(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, d_o):
-        q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
-        if _plain_eager(d_o, q, k, v, o, lse) and _plain_grad(d_o):
+        q, k, v, o, lse, low, cu_seqlens = ctx.saved_tensors
+        if _plain_eager(d_o, q, k, v, o, lse, low) and _plain_grad(d_o):
             need = ctx.needs_input_grad
-            dq, dk, dv = _attn_backward(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale, need[0], need[1] or need[2])
+            dq, dk, dv = _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, ctx.scale, need[0], need[1] or need[2])
             return dq, dk if need[1] else None, dv if need[2] else None, None, None
-        return *_attention_bwd_op(d_o, q, k, v, o, lse, cu_seqlens, ctx.scale), None, None
+        return *_attention_bwd_op(d_o, q, k, v, o, lse, low, cu_seqlens, ctx.scale), None, None
 
     _recorded = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, d_o: _AttentionFn._grads(ctx, d_o)))
 

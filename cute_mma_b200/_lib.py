@@ -161,9 +161,9 @@ def lib() -> ctypes.CDLL:
                 raise RuntimeError(f"{LIB_PATH} lacks {', '.join(missing)}: rebuild it (cute_mma_b200._lib.build(force=True))")
             llp, fl = ctypes.POINTER(ll), ctypes.c_float
             L.prism_attn_fwd.restype = i
-            L.prism_attn_fwd.argtypes = [vp] * 6 + [i] * 7 + [fl, llp, vp, sz, vp]
+            L.prism_attn_fwd.argtypes = [vp] * 7 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_attn_bwd.restype = i
-            L.prism_attn_bwd.argtypes = [vp] * 11 + [i] * 7 + [fl, llp, vp, sz, vp]
+            L.prism_attn_bwd.argtypes = [vp] * 12 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_attn_decode_scratch_bytes.restype = sz
             L.prism_attn_decode_scratch_bytes.argtypes = [i]
             L.prism_attn_decode.restype = i

@@ -455,10 +455,28 @@ __device__ __forceinline__ void attn_zero_tail(char* tile, int valid) {
   __syncwarp();
 }
 
-// One row of `cols` features from TMEM (the thread's lane) times f, rounded once to 16 bits, to global memory in
-// 16-byte pieces.  All threads of the warp call it; only those with `store` write.
-template <int DT, int DH>
-__device__ __forceinline__ void attn_store_row(uint32_t taddr, float f, uint16_t* dst, int dim, bool store) {
+// Four fp32 values as e5m2 bytes, and back.
+__device__ __forceinline__ uint32_t pack_e5m2(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | (uint32_t)hi << 16;
+}
+__device__ __forceinline__ void unpack_e5m2(uint32_t v, float (&f)[4]) {
+  uint32_t a, b;
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(a) : "h"((uint16_t)v));
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(b) : "h"((uint16_t)(v >> 16)));
+  const float2 x = Elem<DT_F16>::unpack(a), y = Elem<DT_F16>::unpack(b);
+  f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+}
+// What rounding to 16 bits took from o is kept times this, which puts it near o's own size.
+template <int DT>
+__device__ __forceinline__ constexpr float low_scale() { return DT == DT_BF16 ? 256.f : 2048.f; }
+
+// One row of `dim` features from TMEM (the thread's lane) times f, rounded once to 16 bits, to global memory in 16-byte
+// pieces; LOW: what the rounding took goes to `low`.  All threads of the warp call it; only those with `store` write.
+template <int DT, int DH, bool LOW>
+__device__ __forceinline__ void attn_store_row(uint32_t taddr, float f, uint16_t* dst, uint8_t* low, int dim, bool store) {
 #pragma unroll
   for (int c = 0; c < DH; c += 32) {
     if (c >= dim) break;
@@ -467,12 +485,38 @@ __device__ __forceinline__ void attn_store_row(uint32_t taddr, float f, uint16_t
     tmem_ld_wait();
 #pragma unroll
     for (int e = 0; e < 32; e += 8) {
-      uint4 v;
-      v.x = Elem<DT>::pack(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f);
-      v.y = Elem<DT>::pack(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
-      v.z = Elem<DT>::pack(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
-      v.w = Elem<DT>::pack(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
-      if (store && c + e < dim) *reinterpret_cast<uint4*>(dst + c + e) = v;
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __uint_as_float(r[e + 2 * i]) * f, y = __uint_as_float(r[e + 2 * i + 1]) * f;
+        v[i] = Elem<DT>::pack(x, y);
+        if constexpr (LOW) {
+          const float2 h = Elem<DT>::unpack(v[i]);
+          r[e + 2 * i] = __float_as_uint((x - h.x) * low_scale<DT>());
+          r[e + 2 * i + 1] = __float_as_uint((y - h.y) * low_scale<DT>());
+        }
+      }
+      if (store && c + e < dim) *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+      if constexpr (LOW) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)   // four to a word, in the first quarter of the registers
+          r[(e + i) / 4] = pack_e5m2(__uint_as_float(r[e + i]), __uint_as_float(r[e + i + 1]), __uint_as_float(r[e + i + 2]),
+                                     __uint_as_float(r[e + i + 3]));
+      }
+    }
+    if constexpr (LOW) {
+      if (store) {
+        if ((dim & 15) == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (c + e * 16 < dim)
+              *reinterpret_cast<uint4*>(low + c + e * 16) = make_uint4(r[e * 4], r[e * 4 + 1], r[e * 4 + 2], r[e * 4 + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e * 8 < dim) *reinterpret_cast<uint2*>(low + c + e * 8) = make_uint2(r[e * 2], r[e * 2 + 1]);
+        }
+      }
     }
   }
 }

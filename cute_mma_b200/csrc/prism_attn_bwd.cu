@@ -31,9 +31,12 @@ constexpr int kThreads = 384, kMathRegs = 208, kOtherRegs = 88;
 #endif
 
 // ---------------------------------------------------------------------------------------------------- delta
-// Sixteen lanes a row of a head: 16-byte pieces of o and do.
+// Sixteen lanes a row of a head: 16-byte pieces of o and do, and 8 bytes of what o's rounding took.  An error of delta is
+// one of every dS of its row with the same sign, which no sum over the keys averages out: with o as rounded alone dq was
+// 0.0025 off (relative norm, 1024 rows, heads of 64, bf16), with the rest 0.0024, of which 0.0023 is the rounding of dS.
 struct DeltaParams {
   const uint16_t *o, *d_o;
+  const uint8_t* low;
   AttnStrides sdo;
   float* delta;
   int heads, dim, len;   // len: rows per batch entry
@@ -57,6 +60,17 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const DeltaParams p) {
       const float2 a = Elem<DT>::unpack(xs[e]), b2 = Elem<DT>::unpack(ys[e]);
       sum = fmaf(a.x, b2.x, fmaf(a.y, b2.y, sum));
     }
+    if (p.low != nullptr) {
+      const uint2 z = *reinterpret_cast<const uint2*>(p.low + unit * p.dim + piece * 8);
+      float f[4], rest = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((e & 1) == 0) unpack_e5m2(e == 0 ? z.x : z.y, f);
+        const float2 b2 = Elem<DT>::unpack(ys[e]);
+        rest = fmaf(f[(e & 1) * 2], b2.x, fmaf(f[(e & 1) * 2 + 1], b2.y, rest));
+      }
+      sum = fmaf(rest, 1.f / low_scale<DT>(), sum);
+    }
   }
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -77,8 +91,10 @@ struct DkvSmem {
   static constexpr int kQ = DH == 128 ? 2 : 4, kDo = DH == 128 ? 3 : 4;   // rings of Q and of dO tiles
   static constexpr uint32_t kBytes = (2 * kKv + kQ + kDo) * kTile + 1024;
 };
+// (Barriers in pairs, used in turn: where one side may be a whole tile ahead of the other, a single one could complete
+// twice before it is looked at.  P of tile i + 2 needs scores that are issued behind the wait for P of tile i.)
 struct DkvBars {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty, clean[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], dp_full, ds_full, acc_full, acc_empty, st_full, st_empty, clean[2];
   uint64_t q_full[4], q_empty[4], do_full[4], do_empty[4];
 };
 
@@ -116,7 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.v_full[s], 1);
       mbar_init(&bars.v_empty[s], 1);
       mbar_init(&bars.s_full[s], 1);
-      mbar_init(&bars.p_full[s], 8);
+      mbar_init(&bars.p_full[s][0], 8);
+      mbar_init(&bars.p_full[s][1], 8);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&bars.q_full[s], 1);
@@ -285,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 2; ++c) {
               // (the next scores' operands are looked for while the second piece is on its way)
               if (c == 1 && !kEarly && more && !arrived(&bars.q_full[nrq.idx], nrq.phase, i)) { ok = false; break; }
-              if (!warp_wait(&bars.p_full[c], cnt & 1)) { ok = false; break; }
+              if (!warp_wait(&bars.p_full[cnt & 1][c], (cnt >> 1) & 1)) { ok = false; break; }
               tc_fence_after_sync();
               if (elect_one())
 #pragma unroll
@@ -359,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.p_full[c]);
+          if (lane == 0) mbar_arrive(&bars.p_full[cnt & 1][c]);
         }
         if (!warp_wait(&bars.dp_full, cnt & 1)) { ok = false; break; }
         tc_fence_after_sync();
@@ -403,8 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row = w.tile * kAttnTile + key;
       const bool mine = row < w.len;
       const long long at = ((w.orow + row) * p.hkv + kvh) * p.dim;
-      if (half == 0) attn_store_row<DT, DH>(tmem + lanes + kDv, 1.f, p.dv + at, p.dim, mine);
-      else attn_store_row<DT, DH>(tmem + lanes + kDk, p.scale, p.dk + at, p.dim, mine);
+      if (half == 0) attn_store_row<DT, DH, false>(tmem + lanes + kDv, 1.f, p.dv + at, nullptr, p.dim, mine);
+      else attn_store_row<DT, DH, false>(tmem + lanes + kDk, p.scale, p.dk + at, nullptr, p.dim, mine);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.acc_empty);
@@ -428,7 +445,7 @@ struct DqSmem {
   static constexpr uint32_t kBytes = (2 * kQ + kK + kV) * kTile + 1024;
 };
 struct DqBars {
-  uint64_t q_full[2], q_empty[2], do_full[2], do_empty[2], s_full, s_read, dp_full[2], ds_full, ds_empty[2], acc_full, acc_empty;
+  uint64_t q_full[2], q_empty[2], do_full[2], do_empty[2], s_full, s_read, dp_full[2], ds_full[2], ds_empty[2], acc_full, acc_empty;
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
 };
 
@@ -460,7 +477,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.ds_empty[1], 1);
     mbar_init(&bars.s_full, 1);
     mbar_init(&bars.s_read, 8);
-    mbar_init(&bars.ds_full, 8);
+    mbar_init(&bars.ds_full[0], 8);
+    mbar_init(&bars.ds_full[1], 8);
     mbar_init(&bars.acc_full, 1);
     mbar_init(&bars.acc_empty, 8);
     mbar_init(&bars.dp_full[0], 1);
@@ -566,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = warp_wait(&bars.acc_empty, (used & 1) ^ 1);
         ++used;
         for (int j = 0; ok && j <= w.tile; ++j, ++cnt, r.next()) {
-          if (!warp_wait(&bars.ds_full, cnt & 1)) { ok = false; break; }
+          if (!warp_wait(&bars.ds_full[cnt & 1], (cnt >> 1) & 1)) { ok = false; break; }
           tc_fence_after_sync();
           const int valid = w.len - j * kAttnTile;
           if (elect_one()) {
@@ -640,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.ds_full);
+        if (lane == 0) mbar_arrive(&bars.ds_full[cnt & 1]);
       }
       if (!ok) break;
       if (!warp_wait(&bars.acc_full, used & 1)) { ok = false; break; }
@@ -649,7 +667,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint16_t* dst = p.dq + ((w.orow + row) * p.hq + head) * p.dim;
       // each warpgroup half of the features
       if (half * (DH / 2) < p.dim)
-        attn_store_row<DT, DH / 2>(tmem + lanes + kDq + half * (DH / 2), p.scale, dst + half * (DH / 2), p.dim - half * (DH / 2), mine);
+        attn_store_row<DT, DH / 2, false>(tmem + lanes + kDq + half * (DH / 2), p.scale, dst + half * (DH / 2), nullptr,
+                                   p.dim - half * (DH / 2), mine);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.acc_empty);
@@ -685,6 +704,7 @@ int launch_attn_bwd(const AttnArgs& a) {
   DeltaParams d;
   d.o = static_cast<const uint16_t*>(a.o);
   d.d_o = static_cast<const uint16_t*>(a.d_o);
+  d.low = a.low;
   d.sdo = a.sdo;
   d.delta = a.delta;
   d.heads = a.hq; d.dim = a.dim; d.rows = a.rows;

@@ -20,6 +20,7 @@ struct FwdParams {
   AttnRows rows;
   uint16_t* o;     // rows x heads x dim
   float* lse;      // heads x rows, c m + log2 l per row, or null
+  uint8_t* low;    // rows x heads x dim, what o's rounding took (e5m2), or null
   int hq, group, dim;
   int pair;        // 1: the two tiles are the same rows of two heads; 0: 256 rows of one head
   float c;         // scale * log2 e
@@ -73,7 +74,7 @@ struct FwdTiles {
 #define PRISM_ATTN_FWD_C0 64
 #endif
 
-template <int DT, int DH>
+template <int DT, int DH, bool LOW>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                     const __grid_constant__ CUtensorMap mv, const FwdParams p) {
@@ -339,7 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const int row = tl.row[t] + r, head = tl.head[t];
       const bool mine = row < w.len;
-      attn_store_row<DT, DH>(o_addr, 1.f / l, p.o + ((w.orow + row) * p.hq + head) * p.dim, p.dim, mine);
+      const long long at = ((w.orow + row) * p.hq + head) * p.dim;
+      attn_store_row<DT, DH, LOW>(o_addr, 1.f / l, p.o + at, LOW ? p.low + at : nullptr, p.dim, mine);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.o_empty[t]);
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int DT, int DH>
 int launch_t(const AttnArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdParams& p) {
-  auto* kern = attn_fwd_kernel<DT, DH>;
+  auto* kern = p.low != nullptr ? attn_fwd_kernel<DT, DH, true> : attn_fwd_kernel<DT, DH, false>;
   if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(kern), FwdSmem<DH>::kBytes, "causal attention")) return rc;
   const unsigned heads = (unsigned)(p.pair ? a.hq / 2 : a.hq);
   kern<<<(unsigned)p.rows.tiles * heads, kThreads, FwdSmem<DH>::kBytes, a.stream>>>(mq, mk, mv, p);
@@ -371,6 +373,7 @@ int launch_attn_fwd(const AttnArgs& a) {
   if (p.rows.tiles == 0) return PRISM_OK;
   p.o = static_cast<uint16_t*>(a.o);
   p.lse = a.lse;
+  p.low = a.low;
   p.c = a.scale * kLog2e;
   p.err = a.err;
   CUtensorMap mq, mk, mv;

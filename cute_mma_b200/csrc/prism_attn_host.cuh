@@ -19,6 +19,7 @@ struct AttnArgs {
   float scale;
   void* o;                    // rows x hq x dim, contiguous (backward: the forward's)
   float* lse;                 // hq x rows, or null (backward: the forward's)
+  uint8_t* low;               // rows x hq x dim, what o's rounding took, or null (backward: the forward's)
   const void* d_o;            // backward: gradient of o with strides sdo
   AttnStrides sdo;
   float* delta;               // backward: scratch hq x rows

@@ -46,18 +46,18 @@ int check_attn(const char* what, const AttnArgs& a, const long long* strides, in
   if (a.rows > 0 && (a.q == nullptr || a.k == nullptr || a.v == nullptr || a.o == nullptr))
     return fail(PRISM_ERR_BAD_ARG, "%s: null tensor", what);
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o) || !aligned16(a.d_o) || !aligned16(a.dq) ||
-      !aligned16(a.dk) || !aligned16(a.dv))
+      !aligned16(a.dk) || !aligned16(a.dv) || !aligned16(a.low))
     return fail(PRISM_ERR_BAD_ARG, "%s: tensors must be 16-byte aligned", what);
   return PRISM_OK;
 }
 
 }  // namespace
 
-extern "C" int prism_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu_seqlens,
-                              int n_seqs, int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+extern "C" int prism_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_low,
+                              const int* cu_seqlens, int n_seqs, int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
                               const long long* strides, void* workspace, size_t workspace_bytes, void* stream) {
   AttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse;
+  a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse; a.low = static_cast<uint8_t*>(o_low);
   a.cu = cu_seqlens; a.n = n_seqs; a.len = seq_len; a.rows = rows;
   a.hq = heads; a.hkv = kv_heads; a.dim = head_dim; a.dtype = dtype; a.scale = scale;
   if (int rc = check_attn("prism_attn_fwd", a, strides, 9)) return rc;
@@ -69,11 +69,12 @@ extern "C" int prism_attn_fwd(const void* q, const void* k, const void* v, void*
 }
 
 extern "C" int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                              void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len,
+                              const void* o_low, void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len,
                               int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
                               const long long* strides, void* workspace, size_t workspace_bytes, void* stream) {
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = const_cast<void*>(o); a.lse = const_cast<float*>(lse); a.d_o = d_o;
+  a.low = const_cast<uint8_t*>(static_cast<const uint8_t*>(o_low));
   a.dq = dq; a.dk = dk; a.dv = dv; a.delta = delta;
   a.cu = cu_seqlens; a.n = n_seqs; a.len = seq_len; a.rows = rows;
   a.hq = heads; a.hkv = kv_heads; a.dim = head_dim; a.dtype = dtype; a.scale = scale;

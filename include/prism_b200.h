@@ -213,15 +213,16 @@ int prism_peer_reduce(const void* const* in_ptrs, void* const* out_ptrs, int wor
  * cu_seqlens (device, n_seqs + 1 int32, or NULL): row ranges of packed sequences; offsets are taken into [0, rows] and
  * never backwards, and rows that belong to no sequence are zeros in every output.  NULL: n_seqs sequences of seq_len rows
  * (rows = n_seqs * seq_len).  strides (host): {batch, row, head} in elements for q, k, v (batch: dense only), multiples of
- * 8; pointers 16-byte aligned.  o: contiguous.  lse: NULL, or heads x rows fp32 for prism_attn_bwd.  The scale is positive.
- * Backward: d_o with strides[9..11], o and lse of the forward; dq, dk, dv contiguous, dq or both of dk and dv NULL where they are
+ * 8; pointers 16-byte aligned.  o: contiguous.  For prism_attn_bwd: lse (heads x rows fp32) and o_low (rows x heads x
+ * head_dim bytes: what rounding o to 16 bits took, as e5m2), each NULL where not wanted.  The scale is positive.
+ * Backward: d_o with strides[9..11], o, lse and o_low (or NULL) of the forward; dq, dk, dv contiguous, dq or both of dk and dv NULL where they are
  * not wanted; delta: scratch, heads x rows fp32.  All sums have one owner: bit-stable.
  * workspace: its status header (PRISM_WORKSPACE_HEADER_BYTES). */
-int prism_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu_seqlens, int n_seqs,
-                   int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+int prism_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_low, const int* cu_seqlens,
+                   int n_seqs, int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
                    const long long* strides, void* workspace, size_t workspace_bytes, void* stream);
 int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                   void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len, int rows,
+                   const void* o_low, void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len, int rows,
                    int heads, int kv_heads, int head_dim, int dtype, float scale, const long long* strides,
                    void* workspace, size_t workspace_bytes, void* stream);
 
