@@ -661,7 +661,8 @@ def run_cfg4(args, dev, rank, world, local_rank):
     plain-mode PrismLinear(group_size=256, reconn_sz=8): R starts as identity blocks, B frozen, R, the
     biases, the layer norms and the embeddings are trained with AdamW on uniformly random token ids;
     global batch 64 sequences, sequences sharded over the ranks, gradients averaged by all-reduce.
-    Attention, norms and the tied LM head are PyTorch ops (outside the Prism path)."""
+    Attention and the norms (with the residual sums before them) are the library's kernels; GELU, the embeddings and the
+    tied LM head with its loss are PyTorch ops."""
     import torch.distributed as dist
     import torch.nn as nn
     import torch.nn.functional as TF
@@ -681,31 +682,30 @@ def run_cfg4(args, dev, rank, world, local_rank):
     class Block(nn.Module):
         def __init__(self):
             super().__init__()
-            self.ln1, self.ln2 = nn.LayerNorm(d), nn.LayerNorm(d)
+            self.ln1, self.ln2 = cp.LayerNorm(d), cp.LayerNorm(d)
             self.qkv, self.proj = plin(d, 3 * d), plin(d, d)
             self.up, self.down = plin(d, 4 * d), plin(4 * d, d)
 
-        def forward(self, x):
-            b, t, _ = x.shape
-            q, k, v = self.qkv(self.ln1(x)).split(d, dim=2)
-            q, k, v = [z.view(b, t, heads, d // heads).transpose(1, 2) for z in (q, k, v)]
-            y = TF.scaled_dot_product_attention(q, k, v, is_causal=True)
-            x = x + self.proj(y.transpose(1, 2).reshape(b, t, d))
-            return x + self.down(TF.gelu(self.up(self.ln2(x))))
+        def forward(self, x, add):
+            """x: the residual stream before ``add``, the output of the block before, has been added to it."""
+            h, x = self.ln1(add, x)
+            q, k, v = self.qkv(h).unflatten(-1, (3 * heads, d // heads)).split(heads, dim=2)
+            h, x = self.ln2(self.proj(cp.causal_attention(q, k, v).flatten(2)), x)
+            return x, self.down(TF.gelu(self.up(h)))
 
     class GPT(nn.Module):
         def __init__(self):
             super().__init__()
             self.wte, self.wpe = nn.Embedding(vocab, d), nn.Embedding(seq, d)
             self.blocks = nn.ModuleList(Block() for _ in range(layers))
-            self.ln_f = nn.LayerNorm(d)
+            self.ln_f = cp.LayerNorm(d)
 
         def forward(self, idx, targets):
             pos = torch.arange(idx.shape[1], device=idx.device)
-            x = self.wte(idx) + self.wpe(pos)
+            x, add = self.wte(idx), self.wpe(pos).expand(*idx.shape, d)
             for blk in self.blocks:
-                x = blk(x)
-            logits = TF.linear(self.ln_f(x), self.wte.weight)   # tied head
+                x, add = blk(x, add)
+            logits = TF.linear(self.ln_f(add, x)[0], self.wte.weight)   # tied head
             return TF.cross_entropy(logits.float().view(-1, vocab), targets.reshape(-1))
 
     torch.manual_seed(0)

@@ -126,7 +126,8 @@ def _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, scale, need_dq=True, n
     dk, dv = (k.new_empty(k.shape) if need_dkv else None for _ in range(2))
     if rows == 0 or not (need_dq or need_dkv):
         return dq, dk, dv
-    o = o.contiguous()
+    # (saved-tensor hooks may have handed back another layout)
+    o, lse, low = o.contiguous(), lse.contiguous(), low.contiguous()
     d_o, sdo = _tma_rows(d_o)
     q, sq = _tma_rows(q)
     k, sk = _tma_rows(k)
@@ -247,9 +248,8 @@ def _check_decode(q, k, v, lengths) -> None:
     for name, t in (("k", k), ("v", v)):
         # (a copy of a whole cache per token is not what a caller wants)
         x, y, z = _steps(t)
-        if t.numel() and (t.stride(-1) != 1 or (x | y | z) & 7 or t.data_ptr() & 15):
-            raise ValueError(f"{name} must have contiguous features, strides that are multiples of 8 elements and start "
-                             "on a 16-byte boundary")
+        if t.numel() and (t.stride(-1) != 1 or (x | y | z) & 7):
+            raise ValueError(f"{name} must have contiguous features and strides that are multiples of 8 elements")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise ValueError("decode_attention has no backward pass; call it under torch.no_grad(), or causal_attention")
 
@@ -272,6 +272,9 @@ def _decode(q, k, v, lengths, scale):
     b, hq, d = q.shape
     if b == 0:
         return o
+    for name, t in (("k", k), ("v", v)):
+        if t.data_ptr() & 15:
+            raise ValueError(f"{name} must start on a 16-byte boundary")
     q, (_, sb, sh) = _tma_rows(q)
     L = _lib.lib()
     with F._device_scope(q.device):

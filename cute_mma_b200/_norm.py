@@ -89,6 +89,7 @@ def _scratch_bytes(L, m, n, device) -> int:
 
 def _norm_backward(dy, dsum, s, weight, stats, need_dbias):
     """(dx, dweight, dbias or None) for the rows s that were normalised."""
+    weight, stats = weight.contiguous(), stats.contiguous()   # (saved-tensor hooks may have handed back another layout)
     dx = s.new_empty(s.shape)
     dw = torch.empty_like(weight)
     db = torch.empty_like(weight) if need_dbias else None

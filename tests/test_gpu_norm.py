@@ -98,3 +98,147 @@ def test_rows_far_from_zero_and_constant_rows():
     x[5] = 7.0
     x[6] = 0.0
     _check(x, w, b, dy, None, None, _run(x, w, b, dy))
+
+
+@gpu
+@pytest.mark.parametrize("n", [768, 1537, 512])
+def test_strided_rows_and_odd_starts(n):
+    m = 200
+    x, w, b, dy, res, ds = _inputs(m, n, torch.bfloat16, torch.bfloat16, seed=n)
+    want = _run(x, w, b, dy, res, ds)
+    wide = lambda t: torch.cat([t, t], 1)[:, :n]
+    got = _run(wide(x), w, b, wide(dy), wide(res), wide(ds))
+    odd = lambda t: torch.empty(m * n + 1, device=DEV, dtype=t.dtype)[1:].view(m, n).copy_(t)
+    got2 = _run(odd(x), w, b, odd(dy), odd(res), odd(ds))
+    flipped = lambda t: t.t().contiguous().t()
+    got3 = _run(flipped(x), w, b, flipped(dy), flipped(res), flipped(ds))
+    for other in (got, got2, got3):
+        for name, i in (("y", 0), ("s", 1), ("dx", 2)):
+            # (rows read in other pieces are summed in another order)
+            assert torch.allclose(other[i].float(), want[i].float(), rtol=2.0 ** -7, atol=2.0 ** -10), name
+        _check(x, w, b, dy, res, ds, other)
+
+
+@gpu
+def test_leading_dimensions_single_values_and_no_rows():
+    x, w, b, dy, _, _ = _inputs(24, 96, torch.float16, torch.float16)
+    y = cp.layer_norm(x, w, b)
+    assert torch.equal(cp.layer_norm(x.view(2, 3, 4, 96), w, b), y.view(2, 3, 4, 96))
+    assert torch.equal(cp.layer_norm(x[5], w, b), y[5])
+    assert cp.layer_norm(x[:0], w, b).shape == (0, 96)
+    e, w1, b1 = x[:0].detach().requires_grad_(), w.detach().requires_grad_(), b.detach().requires_grad_()
+    for g in torch.autograd.grad(cp.layer_norm(e, w1, b1), [e, w1, b1], x[:0])[1:]:
+        assert torch.count_nonzero(g) == 0
+    no_bias = cp.layer_norm(x, w)
+    assert torch.allclose(no_bias.float() + b.float(), y.float(), atol=2e-2)
+
+
+@gpu
+@pytest.mark.parametrize("n", [96, 768, 4096])
+def test_a_spoiled_row_stays_in_its_row(n):
+    x, w, b, dy, _, _ = _inputs(70, n, torch.bfloat16, torch.float32)
+    clean = _run(x, w, b, dy)
+    x[33, 5], dy[20] = float("inf"), float("nan")
+    got = _run(x, w, b, dy)
+    keep = torch.ones(70, dtype=torch.bool, device=DEV)
+    keep[33] = False
+    assert torch.equal(got[0][keep], clean[0][keep]) and torch.isnan(got[0][33]).all()
+    keep[20] = False
+    assert torch.equal(got[2][keep], clean[2][keep]) and torch.isnan(got[2][20]).all()
+    assert torch.isnan(got[3]).all() and torch.isnan(got[4]).all()
+
+
+@gpu
+def test_same_bits_every_time_streams_and_graphs():
+    x, w, b, dy, res, ds = _inputs(3000, 768, torch.bfloat16, torch.float32)
+    first = _run(x, w, b, dy, res, ds)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(_run(x, w, b, dy, res, ds))
+    torch.cuda.synchronize()
+    for got in outs:
+        for a, c in zip(first, got):
+            assert torch.equal(a, c)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b, res)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, s = cp.layer_norm(*leaves[:3], residual=leaves[3])
+        grads = torch.autograd.grad([y, s], leaves[:3], [dy, ds])
+    with torch.no_grad():
+        leaves[0].copy_(x.flip(0))
+        leaves[3].copy_(res.flip(0))
+    dy.copy_(dy.flip(0))
+    ds.copy_(ds.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, first[0].flip(0)) and torch.equal(s, first[1].flip(0)) and torch.equal(grads[0], first[2].flip(0))
+    assert torch.allclose(grads[1], first[3], rtol=1e-4, atol=1e-3)
+
+
+@gpu
+def test_unused_outputs_traced_calls_and_hooks():
+    x, w, b, dy, res, ds = _inputs(50, 264, torch.bfloat16, torch.bfloat16)
+    want = _run(x, w, b, dy, res, ds)
+    l = [t.detach().requires_grad_() for t in (x, w, b, res)]
+    y, s, _ = torch.ops.prism_b200.layer_norm(*l[:3], 1e-5, l[3])
+    got = [y, s, *torch.autograd.grad([y, s], l, [dy, ds])]
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+    y, s = cp.layer_norm(*l[:3], residual=l[3])
+    dx, dr = torch.autograd.grad(s, [l[0], l[3]], ds)
+    assert torch.equal(dx, ds) and torch.equal(dr, ds)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous(), lambda t: t.t()):
+        y, s = cp.layer_norm(*l[:3], residual=l[3])
+    for a, c in zip(torch.autograd.grad([y, s], l[:3], [dy, ds]), want[2:]):
+        assert torch.equal(a, c)
+
+
+@gpu
+def test_gradients_against_differences():
+    """Central differences of the 64-bit forward along directions of unit entries; their third-order rest is below 2^-12
+    of the sum of absolute products for a step of 2^-10."""
+    x, w, b, dy, _, _ = _inputs(30, 200, torch.float16, torch.float32, seed=8)
+    got = _run(x, w, b, dy)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+
+    def loss(x, w, b):
+        return (torch.nn.functional.layer_norm(x, (200,), w, b, 1e-5) * dy.double()).sum()
+
+    base, h = [x.double(), w.double(), b.double()], 2.0 ** -10
+    for i in range(3):
+        e = torch.randn(base[i].shape, device=DEV, generator=gen, dtype=torch.float64).sign()
+        plus, minus = [list(base) for _ in range(2)]
+        plus[i], minus[i] = base[i] + h * e, base[i] - h * e
+        num = (loss(*plus) - loss(*minus)) / (2 * h)
+        g = got[2 + i].double()
+        assert (num - (g * e).sum()).abs() <= (2.0 ** -11 + 2.0 ** -12) * g.abs().sum() + 1e-3
+
+
+@gpu
+def test_module_matches_torch_and_many_rows():
+    a, c = torch.nn.LayerNorm(320, device=DEV), cp.LayerNorm(320, device=DEV)
+    with torch.no_grad():
+        a.weight.normal_(), a.bias.normal_()
+    c.load_state_dict(a.state_dict())
+    x = torch.randn(200000, 320, device=DEV).bfloat16()
+    assert torch.allclose(c(x).float(), a(x.float()), atol=2e-2, rtol=2.0 ** -8)
+    y, s = c(x, x)
+    assert torch.equal(s, x + x) and torch.equal(y, c(s))
+
+
+@gpu
+def test_offsets_past_32_bits():
+    m, n, ld = 70000, 512, 32768
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    buf = torch.zeros(m, ld, device=DEV, dtype=torch.bfloat16)
+    x = buf[:, -n:]
+    x.normal_()
+    _, w, b, dy, _, _ = _inputs(m, n, torch.bfloat16, torch.float32)
+    got, want = _run(x, w, b, dy), _run(x.contiguous(), w, b, dy)
+    for i in (0, 2, 3, 4):
+        assert torch.equal(got[i], want[i])
+    del buf, x
