@@ -179,24 +179,20 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-#ifndef PRISM_ATTN_POLL
-#define PRISM_ATTN_POLL 1
-#endif
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-#if PRISM_ATTN_POLL
-#define ATTN_TEST mbar_test
-#else
-#define ATTN_TEST mbar_try_wait
-#endif
-  if (__all_sync(0xffffffffu, ATTN_TEST(bar, parity))) return true;
+template <bool POLL>
+__device__ __forceinline__ bool warp_wait_t(uint64_t* bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
   const long long t0 = clock64();
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
-      if (__all_sync(0xffffffffu, ATTN_TEST(bar, parity))) return true;
+      if (__all_sync(0xffffffffu, POLL ? mbar_test(bar, parity) : mbar_try_wait(bar, parity))) return true;
     if (__any_sync(0xffffffffu, clock64() - t0 > PRISM_WAIT_LIMIT_CYCLES)) return false;
   }
 }
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return warp_wait_t<true>(bar, parity); }
+// For warps with time to spare, whose polling would only take issue slots from the arithmetic: asleep in try_wait.
+__device__ __forceinline__ bool warp_wait_asleep(uint64_t* bar, uint32_t parity) { return warp_wait_t<false>(bar, parity); }
 
 // The work of a CTA: it begins with the tile of its own block index and then takes over blocks that have not started yet
 // (cluster launch control), so that the loads and first products of the next tile run beside the end of this one and no

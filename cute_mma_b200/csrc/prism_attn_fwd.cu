@@ -21,16 +21,22 @@ struct FwdParams {
   uint16_t* o;     // rows x heads x dim
   float* lse;      // heads x rows, c m + log2 l per row, or null
   uint8_t* low;    // rows x heads x dim, what o's rounding took (e5m2), or null
+  const uint16_t* v;   // as the tensor map has it, for the rows of infinities and NaN
+  AttnStrides sv;
   int hq, group, dim;
   int pair;        // 1: the two tiles are the same rows of two heads; 0: 256 rows of one head
   float c;         // scale * log2 e
   int* err;
 };
 
-// Two softmax warpgroups, and one of the two issuing warps, the loading warp and one that only lends its registers: a
-// softmax thread holds a row of 128 scores.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is
+// Two softmax warpgroups, and one of the two issuing warps, the loading warp and one that looks through values: a softmax
+// thread holds a row of 128 scores.  256 x 208 + 128 x 88 registers = 384 x 168, what the block is
 // launched with.
 constexpr int kThreads = 384, kSoftmaxRegs = 208, kOtherRegs = 88;
+
+// Blocks of keys that are looked through before their product (the tiles' own rows) in turn: at most as many are under way
+// as the ring holds value tiles.
+constexpr int kChecks = 8;
 
 template <int DH>
 struct FwdSmem {
@@ -44,9 +50,12 @@ struct FwdBars {
   uint64_t q_full[2][2], q_empty[2][2], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
   uint64_t turn[2][4];
   uint64_t kv_full[10], kv_empty[10];
+  uint64_t checked[kChecks];
+  int unbounded;   // infinities or NaN were found among checked values, of whatever piece of work
 };
 
-// The two tiles of a piece of work: row offset, head and number of key blocks.
+// The two tiles of a piece of work: row offset, head and number of key blocks.  From block n[0] - 1 on keys stand beside
+// rows that must not see them.
 struct FwdTiles {
   int row[2], head[2], n[2];
   __device__ __forceinline__ FwdTiles(const FwdParams& p, const AttnWork& w, int slot_head) {
@@ -65,6 +74,59 @@ struct FwdTiles {
   }
   __device__ __forceinline__ int most() const { return max(n[0], n[1]); }
 };
+
+// Looks through the first `valid` rows of a value tile, by one warp.  A masked key has the probability 0, but 0 times its
+// infinities and NaN would not be 0: those become zeros here (true: there were any), and the rows that do see them get
+// them at the end (attn_add_unbounded).  (Inlined, like all that runs behind a change of the register share: a called
+// function is compiled without regard to it.)  Rows behind the sequence become zeros up to the next sixteen.
+template <int DT, int DH>
+__device__ __forceinline__ bool attn_check_values(char* tile, int valid) {
+  constexpr uint32_t kExp = DT == DT_BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = DT == DT_BF16 ? 0x00800080u : 0x04000400u;
+  const int lane = threadIdx.x & 31;
+  if (valid < kAttnTile) attn_zero_tail<DH>(tile, valid);
+  const int pieces = min(valid, kAttnTile) * 8;   // of 16 bytes, of one 64-feature half
+  uint32_t sum[4] = {0u, 0u, 0u, 0u};   // of zero times every value: zero, or NaN
+#pragma unroll 1
+  for (int s = 0; s < DH / 64; ++s) {
+    const uint4* t = reinterpret_cast<const uint4*>(tile + s * kAttnSub);
+#pragma unroll 8
+    for (int i = lane; i < pieces; i += 32) {
+      const uint4 x = t[i];
+      sum[0] = Pk<DT>::fma(x.x, 0u, sum[0]);
+      sum[1] = Pk<DT>::fma(x.y, 0u, sum[1]);
+      sum[2] = Pk<DT>::fma(x.z, 0u, sum[2]);
+      sum[3] = Pk<DT>::fma(x.w, 0u, sum[3]);
+    }
+  }
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (sum[i] & kExp) + kOne;   // (an exponent of ones overflows into the bit above)
+  if (!__any_sync(0xffffffffu, any & 0x80008000u)) return false;
+  for (int s = 0; s < DH / 64; ++s) {
+    uint32_t* t = reinterpret_cast<uint32_t*>(tile + s * kAttnSub);
+    for (int i = lane; i < pieces * 4; i += 32) {
+      const uint32_t c = (t[i] & kExp) + kOne;
+      if (c & 0x8000u) t[i] &= 0xffff0000u;
+      if (c & 0x80000000u) t[i] &= 0x0000ffffu;
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  return true;
+}
+// o += the infinities and NaN among the values that row `row` of the sequence sees, from row `first` on.
+template <int DT>
+__device__ __forceinline__ void attn_add_unbounded(const FwdParams& p, const AttnWork& w, int first, int row, int kvh, uint16_t* o) {
+#pragma unroll 1
+  for (int j = first; j <= row; ++j) {
+    const uint16_t* v = p.v + w.batch * p.sv.batch + (long long)(w.row + j) * p.sv.row + kvh * p.sv.head;
+#pragma unroll 1
+    for (int d = 0; d < p.dim; ++d) {
+      const float x = Elem<DT>::unpack(v[d]).x;
+      if (!isfinite(x)) o[d] = (uint16_t)(Elem<DT>::pack(Elem<DT>::unpack(o[d]).x + x, 0.f) & 0xffffu);
+    }
+  }
+}
 
 // Every kPolyOf-th pair of exponentials goes to the FMA pipe.
 #ifndef PRISM_ATTN_FWD_POLY
@@ -93,7 +155,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc_cta(&tmem_slot, 512);
     tmem_relinquish_cta();
   } else if (warp == 9 && lane == 0) {
-    attn_sched_init(sched, 10);
+    attn_sched_init(sched, 11);
+    for (int i = 0; i < kChecks; ++i) mbar_init(&bars.checked[i], 1);
+    bars.unbounded = 0;
     for (int t = 0; t < 2; ++t) {
       for (int i = 0; i < 4; ++i) mbar_init(&bars.turn[t][i], 1);
       for (int i = 0; i < 2; ++i) {
@@ -110,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < L::kRing; ++s) {
       mbar_init(&bars.kv_full[s], 1);
-      mbar_init(&bars.kv_empty[s], 2);
+      mbar_init(&bars.kv_empty[s], 3);
     }
     fence_mbar_init();
   }
@@ -166,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_tile = smem_u32(smem) + t * L::kTile, ring = smem_u32(smem) + 2 * L::kQ * L::kTile;
       const uint32_t st = tmem + t * 128, ot = tmem + kO + t * DH, pt = kEarly ? tmem + 256 + t * 64 : st;
       Ring rk(L::kRing), rq(L::kQ);
-      uint32_t used = 0, made = 0, blocks = 0;   // pieces of work, scores and key blocks so far
+      uint32_t used = 0, made = 0, blocks = 0, checks = 0;   // pieces of work, scores, key blocks and checked ones so far
       auto scores = [&](bool last) {
         tc_fence_after_sync();
         if (elect_one()) {
@@ -182,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = tl.most(), nt = tl.n[t];
         ok = warp_wait(&bars.q_full[t][rq.idx], rq.phase);
         if (ok && nt == 0 && elect_one()) mbar_arrive(&bars.q_empty[t][rq.idx]);
-        // every lane waits (the warp stays together for the zeros of a last tile), one issues
+        // every lane waits, one issues
         for (int j = -1; ok && j < n; ++j) {
           // scores of block j + 1, where they need not wait for block j's product
           Ring rv = rk;   // (for j >= 0: stands on K of block j + 1, V of block j before it)
@@ -200,12 +264,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (j >= 0) {
             if (!warp_wait(&bars.kv_full[rv.idx], rv.phase)) { ok = false; break; }
+            if (j >= tl.n[0] - 1) {
+              if (!warp_wait(&bars.checked[checks % kChecks], (checks / kChecks) & 1)) { ok = false; break; }
+              ++checks;
+            }
             if (j >= nt) {
               if (elect_one()) mbar_arrive(&bars.kv_empty[rv.idx]);
             } else {
               const int valid = w.len - j * kAttnTile;
               const int steps = valid >= kAttnTile ? 8 : (valid + 15) >> 4;
-              if (valid < kAttnTile) attn_zero_tail<DH>(smem + (2 * L::kQ + rv.idx) * L::kTile, valid);   // (both warps, the same zeros)
               const uint32_t v_tile = ring + rv.idx * L::kTile;
               if (j == 0 && !warp_wait(&bars.o_empty[t], (used & 1) ^ 1)) { ok = false; break; }
               if (!warp_wait(&bars.p_full[t][0], blocks & 1)) { ok = false; break; }
@@ -232,6 +299,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         used += nt > 0;
         rq.next();
+      }
+    } else {
+      // the warp that looks through the values of the tiles' own rows
+      Ring r(L::kRing);
+      uint32_t checks = 0;
+      while (ok && attn_next(sched, rw, &w, &slot_head, &ok)) {
+        const FwdTiles tl(p, w, slot_head);
+        const int n = tl.most();
+        // (it sees every tile of the ring and gives it back like the issuing warps: a barrier's parity says nothing to one
+        // that has left out a phase)
+        for (int i = 0; i < 2 * n; ++i, r.next()) {
+          const int j = i >> 1;
+          if (!warp_wait_asleep(&bars.kv_full[r.idx], r.phase)) { ok = false; break; }
+          if ((i & 1) && j >= tl.n[0] - 1) {
+            const bool found = attn_check_values<DT, DH>(smem + (2 * L::kQ + r.idx) * L::kTile, w.len - j * kAttnTile);
+            if (lane == 0) {
+              if (found) bars.unbounded = 1;
+              mbar_arrive(&bars.checked[checks % kChecks]);
+            }
+            ++checks;
+          }
+          if (lane == 0) mbar_arrive(&bars.kv_empty[r.idx]);
+        }
       }
     }
   } else {
@@ -289,9 +379,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // (a NaN among the scores makes the comparison fail and m NaN: the whole row is NaN then.  A row at -infinity
         // has NaN on its left side as well, and nothing to rescale.)
-        if (__any_sync(0xffffffffu, !((mnew - m) * p.c <= 8.f))) {
-          const float f = ex2((m - (mnew == -INFINITY ? 0.f : mnew)) * p.c);
-          m = mnew;
+        const bool grown = !((mnew - m) * p.c <= 8.f);
+        if (__any_sync(0xffffffffu, grown)) {
+          // (each row by its own maximum alone: its bits do not depend on its neighbours)
+          const float f = grown ? ex2((m - (mnew == -INFINITY ? 0.f : mnew)) * p.c) : 1.f;
+          if (grown) m = mnew;
           l *= f;
           if (j > 0) {
 #pragma unroll
@@ -345,6 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.o_empty[t]);
+      if (*static_cast<volatile int*>(&bars.unbounded) && mine)
+        attn_add_unbounded<DT>(p, w, (tl.n[0] - 1) * kAttnTile, row, head / p.group, p.o + at);
       if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + lg2(l);
     }
   }
@@ -374,6 +468,8 @@ int launch_attn_fwd(const AttnArgs& a) {
   p.o = static_cast<uint16_t*>(a.o);
   p.lse = a.lse;
   p.low = a.low;
+  p.v = static_cast<const uint16_t*>(a.v);
+  p.sv = a.sv;
   p.c = a.scale * kLog2e;
   p.err = a.err;
   CUtensorMap mq, mk, mv;

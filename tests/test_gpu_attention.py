@@ -369,3 +369,34 @@ def test_empty_calls_and_offsets_out_of_range():
         _run(q, k, v, do, torch.tensor(bad, device=DEV, dtype=torch.int32))
     torch.cuda.synchronize()
     cp.check_device_status()
+
+
+@gpu
+@pytest.mark.parametrize("heads", [(4, 2, 64), (3, 3, 64), (4, 2, 128), (3, 1, 80)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_what_later_rows_hold_does_not_reach_earlier_ones(heads, dt):
+    """Infinities and NaN in the keys and values of later rows of the same sequence (a padded batch holds anything behind
+    its lengths): earlier rows keep their bits, rows from there on are what the formula makes of them."""
+    hq, hkv, d = heads
+    n = 300
+    q, k, v, _ = _inputs((n,) * 3, hq, hkv, d, dt, seed=d)
+    q, k, v = [t.view(3, n, *t.shape[1:]) for t in (q, k, v)]
+    clean = cp.causal_attention(q, k, v)
+    at = (5, 140, 270)
+    for b, i in enumerate(at):
+        k[b, i + 1:], v[b, i + 1:], q[b, i + 1:] = float("nan"), float("nan"), float("nan")
+    got = cp.causal_attention(q, k, v)
+    for b, i in enumerate(at):
+        assert torch.equal(got[b, :i + 1], clean[b, :i + 1])
+        assert torch.isnan(got[b, i + 1:]).all()
+    q, k, v, _ = _inputs((n,), hq, hkv, d, dt, seed=d)
+    v[20, 0, 3], v[150, 0, 3], v[299, 0, 5], v[33, 0, 1] = float("inf"), float("-inf"), float("nan"), float("-inf")
+    got = cp.causal_attention(q, k, v).float()
+    g = hq // hkv
+    assert torch.isfinite(got[:20, :g]).all() and (got[20:150, :g, 3] == float("inf")).all() and torch.isnan(got[150:, :g, 3]).all()
+    assert (got[33:, :g, 1] == float("-inf")).all() and torch.isfinite(got[:33, :g, 1]).all() and torch.isnan(got[299, :g, 5]).all()
+    rest = got.clone()
+    rest[:, :g, 1] = rest[:, :g, 3] = 0
+    rest[299, :g, 5] = 0
+    assert torch.isfinite(rest).all()
+    cp.check_device_status()
