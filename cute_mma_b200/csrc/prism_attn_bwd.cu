@@ -417,11 +417,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!warp_wait(&bars.acc_full, used & 1)) { ok = false; break; }
       ++used;
       tc_fence_after_sync();
-      const int row = w.tile * kAttnTile + key;
-      const bool mine = row < w.len;
-      const long long at = ((w.orow + row) * p.hkv + kvh) * p.dim;
-      if (half == 0) attn_store_row<DT, DH, false>(tmem + lanes + kDv, 1.f, p.dv + at, nullptr, p.dim, mine);
-      else attn_store_row<DT, DH, false>(tmem + lanes + kDk, p.scale, p.dk + at, nullptr, p.dim, mine);
+      const int row0 = w.tile * kAttnTile + key - lane;
+      const long long at = ((w.orow + row0) * p.hkv + kvh) * p.dim, step = (long long)p.hkv * p.dim;
+      if (half == 0) attn_store_rows<DT, DH, false>(tmem + lanes + kDv, 1.f, p.dv + at, nullptr, step, p.dim, w.len - row0);
+      else attn_store_rows<DT, DH, false>(tmem + lanes + kDk, p.scale, p.dk + at, nullptr, step, p.dim, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.acc_empty);
@@ -664,11 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!warp_wait(&bars.acc_full, used & 1)) { ok = false; break; }
       ++used;
       tc_fence_after_sync();
-      uint16_t* dst = p.dq + ((w.orow + row) * p.hq + head) * p.dim;
-      // each warpgroup half of the features
-      if (half * (DH / 2) < p.dim)
-        attn_store_row<DT, DH / 2, false>(tmem + lanes + kDq + half * (DH / 2), p.scale, dst + half * (DH / 2), nullptr,
-                                   p.dim - half * (DH / 2), mine);
+      const int row0 = row - lane, part = half * (DH / 2);   // (each warpgroup half of the features)
+      if (part < p.dim)
+        attn_store_rows<DT, DH / 2, false>(tmem + lanes + kDq + part, p.scale, p.dq + ((w.orow + row0) * p.hq + head) * p.dim + part,
+                                           nullptr, (long long)p.hq * p.dim, p.dim - part, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.acc_empty);

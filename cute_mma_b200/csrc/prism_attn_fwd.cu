@@ -432,13 +432,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const int row = tl.row[t] + r, head = tl.head[t];
       const bool mine = row < w.len;
-      const long long at = ((w.orow + row) * p.hq + head) * p.dim;
-      attn_store_row<DT, DH, LOW>(o_addr, 1.f / l, p.o + at, LOW ? p.low + at : nullptr, p.dim, mine);
+      const int row0 = row - lane;
+      const long long at = ((w.orow + row0) * p.hq + head) * p.dim, step = (long long)p.hq * p.dim;
+      attn_store_rows<DT, DH, LOW>(o_addr, 1.f / l, p.o + at, LOW ? p.low + at : nullptr, step, p.dim, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.o_empty[t]);
+      __syncwarp();   // (its row was stored by the lanes beside it)
       if (*static_cast<volatile int*>(&bars.unbounded) && mine)
-        attn_add_unbounded<DT>(p, w, (tl.n[0] - 1) * kAttnTile, row, head / p.group, p.o + at);
+        attn_add_unbounded<DT>(p, w, (tl.n[0] - 1) * kAttnTile, row, head / p.group, p.o + at + lane * step);
       if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + lg2(l);
     }
   }
