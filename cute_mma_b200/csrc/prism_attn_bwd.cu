@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);   // (known to be the same in all lanes)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (dq's CTAs may follow where SMs run out of this work)
   bool ok = true;
   AttnWork w;
   int kvh;
@@ -673,6 +674,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);
+  // nothing here needs dk and dv, but the launch must not count as done before theirs is
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 8) tmem_dealloc_cta(tmem, 512);
@@ -691,7 +694,18 @@ int launch_t(const AttnArgs& a, const CUtensorMap* m, BwdParams p) {
   if (int rc = attn_rows(a, kAttnTile, a.hq, &p.rows)) return rc;
   auto* dq = attn_bwd_dq_kernel<DT, DH>;
   if (int rc = set_max_dynamic_smem(reinterpret_cast<const void*>(dq), DqSmem<DH>::kBytes, "causal attention dq")) return rc;
-  dq<<<(unsigned)p.rows.tiles * (unsigned)a.hq, kThreads, DqSmem<DH>::kBytes, a.stream>>>(m[0], m[1], m[2], m[3], p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.rows.tiles * (unsigned)a.hq);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = DqSmem<DH>::kBytes;
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.dk != nullptr;   // behind dk and dv's launch only: that one started when delta was there
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, dq, m[0], m[1], m[2], m[3], p);
+  if (e != cudaSuccess) return fail(PRISM_ERR_CUDA, "causal attention dq: launch failed: %s", cudaGetErrorString(e));
   return check_launch("causal attention dq");
 }
 
