@@ -297,30 +297,17 @@ __device__ __forceinline__ bool attn_next(AttnSched& s, Ring& r, AttnWork* w, in
   return w->tile >= 0;
 }
 
-// 2^x for two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], a polynomial of degree 5 for 2^f (least largest
-// relative error with the constant fixed to 1, by linear programming: 1.9e-7 in fp32) times 2^n.  Below 2^-126 the result
-// stays at 2^-126 (of a largest probability of 1); NaN stays NaN.  The special function unit makes 16 of these a clock and
-// SM, a quarter of what one tile of 128 x 128 scores per 1024 clocks of products needs together with the rest: part of
-// the exponentials are done here.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t"
-      ".reg .b64 ra, rb, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\t"
-      "mov.b64 rb, {%4, %5};\n\t"
-      "add.rn.f32x2 rd, ra, rb;\n\t"
-      "mov.b64 {%0, %1}, rd;\n\t"
-      "}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// 2^x for two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], a polynomial of degree 5 for 2^f (least largest
+// relative error with the constant fixed to 1, by linear programming: 1.9e-7 in fp32) times 2^n.  Below 2^-126 the result
+// stays at 2^-126 (of a largest probability of 1); NaN stays NaN.  The special function unit makes 16 of these a clock and
+// SM: 1024 clocks for a tile of 128 x 128, as long as two products take with heads of 128.  The backward kernels do a quarter of
+// them here (8192 rows, 16 heads: dk and dv 526 -> 508 us with heads of 128, 400 -> 386 us with heads of 64; dq 314 -> 309
+// and 253 -> 231 us).  The forward kernel, which issues more beside them, does not: 253 -> 264 and 199 -> 204 us with an eighth.
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
   const float2 t = add2(x, both(12582912.f));                       // n in the low bits

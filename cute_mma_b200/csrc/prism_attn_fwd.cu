@@ -6,9 +6,14 @@
 // (every p stays below 2^8, which costs neither 16-bit type any of its digits); the end divides by l.
 // A CTA works on two 128-row tiles at a time with a warpgroup each (two heads of a group, whose keys are the same, or 256
 // rows of one head), so that the tensor core has the other tile's products while a warpgroup is in its exponentials.
-// P is handed over in halves: the first half's product runs beside the second half's exponentials.  Keys and values pass
+// P is handed over in two pieces: the first one's product runs beside the second one's exponentials.  Keys and values pass
 // through one ring of shared tiles.  TMEM, heads of up to 64: S of both tiles, P of both, O of both, so that the next
 // scores are formed as soon as these have been read; wider heads: P takes the place of S, which waits for P V.
+//
+// Measured, bf16, one sequence of 8192 rows, 16 heads: of 128, 253 us, 1086 TFLOP/s of the causal half's products (of a
+// measured 1655), tensor pipe 53 % and special function unit 53 % busy: bound by the chain S -> P -> O of a tile, which
+// two tiles of a CTA overlap in part; of 64, 190 us, 723 TFLOP/s, special function unit 66 %: bound by the exponentials,
+// which take the unit twice as long as both products take the tensor core.
 #include "prism_attn.cuh"
 #include "prism_host.cuh"
 #include "prism_attn_host.cuh"
@@ -114,6 +119,7 @@ __device__ __forceinline__ bool attn_check_values(char* tile, int valid) {
   __syncwarp();
   return true;
 }
+
 // o += the infinities and NaN among the values that row `row` of the sequence sees, from row `first` on.
 template <int DT>
 __device__ __forceinline__ void attn_add_unbounded(const FwdParams& p, const AttnWork& w, int first, int row, int kvh, uint16_t* o) {
@@ -128,14 +134,6 @@ __device__ __forceinline__ void attn_add_unbounded(const FwdParams& p, const Att
   }
 }
 
-// Every kPolyOf-th pair of exponentials goes to the FMA pipe.
-#ifndef PRISM_ATTN_FWD_POLY
-#define PRISM_ATTN_FWD_POLY 1000
-#endif
-#ifndef PRISM_ATTN_FWD_C0
-#define PRISM_ATTN_FWD_C0 64
-#endif
-
 template <int DT, int DH, bool LOW>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -143,7 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = FwdSmem<DH>;
   constexpr bool kEarly = DH == 64;   // S does not share its columns with P
   constexpr uint32_t kO = kEarly ? 384 : 256;
-  constexpr int kFirst = PRISM_ATTN_FWD_C0;   // keys of P's first piece
+  // keys of P's first piece (8192 rows, 16 heads: of 64, 201 / 199 / 190 us with 32 / 64 / 96; of 128, 262 / 253 / 262)
+  constexpr int kFirst = kEarly ? 96 : 64;
   extern __shared__ uint8_t smem_raw[];
   __shared__ FwdBars bars;
   __shared__ AttnSched sched;
@@ -407,9 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 128; e += 2) {
           const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, n2);
-          float2 y;
-          if ((e / 2) % PRISM_ATTN_FWD_POLY == PRISM_ATTN_FWD_POLY - 1) y = ex2_poly2(x);
-          else y = make_float2(ex2(x.x), ex2(x.y));
+          const float2 y = make_float2(ex2(x.x), ex2(x.y));
           if (e & 2) sum1 = add2(sum1, y);
           else sum0 = add2(sum0, y);
           s[e >> 1] = Elem<DT>::pack(y.x, y.y);   // pairs land in the first half of the registers

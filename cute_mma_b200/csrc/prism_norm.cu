@@ -3,6 +3,8 @@
 //   y = xh w + b;   g = dy w, dx = rstd (g - mean g - xh mean(g xh)) (+ ds), dw = sum over rows of dy xh, db = sum of dy.
 // Bound by HBM: every element is read once and kept in registers (16 to 32 a thread) between the two sums of a row.  The
 // squares are taken of deviations from the mean, not as a difference of means, which would lose rows far from zero.
+// Measured, bf16, 16384 rows of 4096 with a residual (cold L2): forward 82 us for 537 MB, 6.5 TB/s, as fast as a copy;
+// backward 83 us for 537 MB and the weight gradients' second launch.  Rows of 768: 20.5 and 27.6 us for 101 MB.
 //
 // The threads of a row are 8 to 512, the first that hold its columns; up to 32 they are part of a warp and reduce by
 // shuffles, several rows to a CTA.  Rows of full 16-byte pieces move in those, others in pairs or singly.
@@ -11,11 +13,6 @@
 
 namespace prism {
 namespace {
-
-template <int DT>
-__device__ __forceinline__ float to_float(uint16_t v) {
-  return Elem<DT>::unpack((uint32_t)v).x;
-}
 
 // VEC consecutive 16-bit values as packed words (VEC 1: one value in the low half).
 template <int VEC>
@@ -45,7 +42,7 @@ __device__ __forceinline__ void store_piece(uint16_t* p, const Piece<VEC>& v) {
 template <int DT, int VEC>
 __device__ __forceinline__ void widen(const Piece<VEC>& v, float (&f)[VEC]) {
   if constexpr (VEC == 1) {
-    f[0] = to_float<DT>((uint16_t)v.w[0]);
+    f[0] = Elem<DT>::unpack(v.w[0]).x;
   } else {
 #pragma unroll
     for (int e = 0; e < VEC / 2; ++e) {
@@ -158,20 +155,6 @@ __device__ __forceinline__ void load_params(const void* p, bool f32, int t, int 
     }
   }
 }
-__device__ __forceinline__ float2 add2f(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t"
-      ".reg .b64 ra, rb, rd;\n\t"
-      "mov.b64 ra, {%2, %3};\n\t"
-      "mov.b64 rb, {%4, %5};\n\t"
-      "add.rn.f32x2 rd, ra, rb;\n\t"
-      "mov.b64 {%0, %1}, rd;\n\t"
-      "}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
 // ---------------------------------------------------------------------------------------------------- forward
 template <int TPR>
@@ -203,17 +186,17 @@ __global__ void __launch_bounds__(fwd_threads<TPR>()) norm_fwd_kernel(const Norm
     }
   }
   widen_all<DT, VEC, E>(s, f);
-  float2 acc = twice(0.f);
+  float2 acc = both(0.f);
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) acc = add2f(acc, f[e]);
+  for (int e = 0; e < E / 2; ++e) acc = add2(acc, f[e]);
   float sum[1] = {acc.x + acc.y};
   row_sum<TPR, 1>(sum, red, 0);
   const float mean = sum[0] / (float)a.cols;
-  acc = twice(0.f);
-  const float2 neg = twice(-mean);
+  acc = both(0.f);
+  const float2 neg = both(-mean);
 #pragma unroll
   for (int e = 0; e < E / 2; ++e) {
-    f[e] = add2f(f[e], neg);
+    f[e] = add2(f[e], neg);
     // (columns behind the row do not count; a pair may hold the row's last one)
     const int col = VEC == 1 ? 2 * e * TPR + t : ((2 * e / VEC) * TPR + t) * VEC + 2 * e % VEC;
     const int next = VEC == 1 ? col + TPR : col + 1;
@@ -231,7 +214,7 @@ __global__ void __launch_bounds__(fwd_threads<TPR>()) norm_fwd_kernel(const Norm
     a.rstd[row] = rstd;
   }
   uint16_t* y = static_cast<uint16_t*>(a.y) + row * a.cols;
-  const float2 r2 = twice(rstd);
+  const float2 r2 = both(rstd);
 #pragma unroll
   for (int i = 0; i < E / VEC; ++i) {
     const int col = (i * TPR + t) * VEC;
@@ -292,7 +275,7 @@ __global__ void __launch_bounds__(bwd_threads<TPR>(), (E == 8 ? 768 : 512) / bwd
   float2 w[E / 2], dw[E / 2], db[E / 2];
   load_params<DT, VEC, E, TPR>(a.weight, a.w_f32, t, a.cols, w);
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) dw[e] = db[e] = twice(0.f);
+  for (int e = 0; e < E / 2; ++e) dw[e] = db[e] = both(0.f);
   const float inv = 1.f / (float)a.cols;
   const long long step = (long long)gridDim.x * kRows;
   const bool with_ds = a.dsum != nullptr;
@@ -345,28 +328,28 @@ __global__ void __launch_bounds__(bwd_threads<TPR>(), (E == 8 ? 768 : 512) / bwd
     const float mean = next_mean, rstd = next_rstd;
     next_mean = row + step < a.rows ? a.mean[row + step] : 0.f;
     next_rstd = row + step < a.rows ? a.rstd[row + step] : 0.f;
-    const float2 r2 = twice(rstd), neg = twice(-mean);
-    float2 h[E / 2], q[E / 2], c0 = twice(0.f), c1 = twice(0.f);
+    const float2 r2 = both(rstd), neg = both(-mean);
+    float2 h[E / 2], q[E / 2], c0 = both(0.f), c1 = both(0.f);
     widen_all<DT, VEC, E>(s, h);
     widen_all<DT, VEC, E>(d, q);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
-      h[e] = mul2(add2f(h[e], neg), r2);
+      h[e] = mul2(add2(h[e], neg), r2);
       dw[e] = fma2(q[e], h[e], dw[e]);
-      db[e] = add2f(db[e], q[e]);
+      db[e] = add2(db[e], q[e]);
       q[e] = mul2(q[e], w[e]);
-      c0 = add2f(c0, q[e]);
+      c0 = add2(c0, q[e]);
       c1 = fma2(q[e], h[e], c1);
     }
     float c[2] = {c0.x + c0.y, c1.x + c1.y};
     row_sum<TPR, 2>(c, red, slot);
     if (!live) continue;
-    const float2 m0 = twice(-c[0] * inv), m1 = twice(-c[1] * inv);
+    const float2 m0 = both(-c[0] * inv), m1 = both(-c[1] * inv);
     uint16_t* dx = static_cast<uint16_t*>(a.dx) + row * a.cols;
     float2 add[E / 2];
     widen_all<DT, VEC, E>(z, add);
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) q[e] = fma2(fma2(h[e], m1, add2f(q[e], m0)), r2, add[e]);
+    for (int e = 0; e < E / 2; ++e) q[e] = fma2(fma2(h[e], m1, add2(q[e], m0)), r2, add[e]);
 #pragma unroll
     for (int i = 0; i < E / VEC; ++i) {
       const int col = (i * TPR + t) * VEC;
