@@ -16,6 +16,7 @@ from . import _functional as F
 from . import _lib
 from ._module import _plain_eager, _plain_grad
 
+_MOST_ROWS = (1 << 31) - 257   # (the kernels' row numbers, rounded up to whole tiles, are 32-bit)
 _STRIDES8, _STRIDES9, _STRIDES12 = (ctypes.c_longlong * n for n in (8, 9, 12))
 
 
@@ -56,8 +57,8 @@ def _check_prompt(q, k, v, cu_seqlens) -> None:
     _check_heads(q, k, v)
     if q.shape[:-2] != k.shape[:-2]:
         raise ValueError(f"q and k must have the same rows, got {tuple(q.shape[:-2])} and {tuple(k.shape[:-2])}")
-    if q.shape[:-2].numel() >= 1 << 31:
-        raise ValueError("more than 2^31 rows")
+    if q.shape[:-2].numel() > _MOST_ROWS:
+        raise ValueError(f"more than {_MOST_ROWS} rows")
     if cu_seqlens is None:
         return
     if q.dim() != 3:
@@ -240,8 +241,8 @@ def _check_decode(q, k, v, lengths) -> None:
     _check_heads(q, k, v)
     if q.shape[0] != k.shape[0]:
         raise ValueError(f"q and k must have the same sequences, got {q.shape[0]} and {k.shape[0]}")
-    if k.shape[1] >= 1 << 31 or q.shape[0] * q.shape[1] >= 1 << 31:
-        raise ValueError("more than 2^31 rows")
+    if k.shape[1] > _MOST_ROWS or q.shape[0] * q.shape[1] > _MOST_ROWS:
+        raise ValueError(f"more than {_MOST_ROWS} rows")
     if (lengths.dtype != torch.int32 or lengths.shape != (q.shape[0],) or not lengths.is_contiguous()
             or lengths.device != q.device):
         raise ValueError("lengths must be a contiguous int32 tensor (sequences,) on the device of q")

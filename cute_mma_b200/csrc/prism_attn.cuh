@@ -38,12 +38,14 @@ __device__ __forceinline__ int attn_clamp(int x, int lo, int hi) { return min(ma
 // are taken into [0, rows] and never run backwards, whatever the tensor holds.  Up to 32 kOwn sequences (a lane keeps
 // kOwn tile counts for as long as the CTA lives) are gone through by levels: a sequence of nt tiles has one each of cost
 // 1 to nt, the tiles of cost above L number sum max(0, nt - L), and a binary search finds the level of idx.  More
-// sequences come in their own order (a search by scanning; with so many no single one weighs much).
+// sequences come in their own order (a search by scanning from where the last one ended; with so many no single one
+// weighs much).
 constexpr int kOwn = 8;
 struct AttnOrder {
   int nt[kOwn];
   int total, most;   // packed, by levels: all tiles, tiles of the longest sequence
   bool levels;
+  int from, before;  // packed, by scanning: where the last search ended, and the tiles before it
 };
 __device__ __forceinline__ void attn_range(const AttnRows& r, int b, int* s, int* e) {
   *s = attn_clamp(__ldg(r.cu + b), 0, r.rows);
@@ -52,6 +54,7 @@ __device__ __forceinline__ void attn_range(const AttnRows& r, int b, int* s, int
 __device__ __forceinline__ AttnOrder attn_order(const AttnRows& r, int bm) {
   AttnOrder o;
   o.levels = r.cu != nullptr && r.n <= 32 * kOwn;
+  o.from = o.before = 0;
   int sum = 0, top = 0;
 #pragma unroll
   for (int k = 0; k < kOwn; ++k) {
@@ -69,7 +72,7 @@ __device__ __forceinline__ AttnOrder attn_order(const AttnRows& r, int bm) {
   o.most = __reduce_max_sync(0xffffffffu, top);
   return o;
 }
-__device__ __forceinline__ AttnWork attn_find(const AttnRows& r, const AttnOrder& o, int idx, int bm, bool late) {
+__device__ __forceinline__ AttnWork attn_find(const AttnRows& r, AttnOrder& o, int idx, int bm, bool late) {
   AttnWork w;
   w.spare = w.n_spare = 0;
   if (r.cu == nullptr) {
@@ -119,7 +122,9 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, const AttnOrder
       }
     }
   } else {
-    for (int b0 = 0; b0 < r.n; b0 += 32) {
+    if (idx < o.before) o.from = o.before = 0;
+    base = o.before;
+    for (int b0 = o.from; b0 < r.n; b0 += 32) {
       const int b = b0 + lane;
       int s = 0, e = 0;
       if (b < r.n) attn_range(r, b, &s, &e);
@@ -132,6 +137,8 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, const AttnOrder
       }
       const unsigned hit = __ballot_sync(0xffffffffu, idx < base + incl);
       if (hit) {
+        o.from = b0;
+        o.before = base;
         const int l = __ffs(hit) - 1;
         const int t = idx - base - (incl - nt);
         w.tile = __shfl_sync(0xffffffffu, late ? nt - 1 - t : t, l);
@@ -244,7 +251,7 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
   uint32_t phase = 0;
   int idx = blockIdx.x;
   bool ok = true;
-  const AttnOrder order = attn_order(rows, bm);
+  AttnOrder order = attn_order(rows, bm);
   while (ok && idx >= 0) {
     const int head = idx % heads;
     const AttnWork w = attn_find(rows, order, idx / heads, bm, late);

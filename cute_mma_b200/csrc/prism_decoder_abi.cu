@@ -27,9 +27,12 @@ int num_sms() {   // of the current device; 148 without one
   return n;
 }
 
+constexpr int kMostRows = 0x7fffffff - 256;   // (row numbers rounded up to whole tiles are ints)
+
 AttnStrides strides_at(const long long* s, int i) { return AttnStrides{s[3 * i], s[3 * i + 1], s[3 * i + 2]}; }
 
 int check_attn(const char* what, const AttnArgs& a, const long long* strides, int n_strides) {
+  if (a.rows > kMostRows) return fail(PRISM_ERR_UNSUPPORTED, "%s: more than %d rows", what, kMostRows);
   if (a.n < 1 || a.len < 0 || a.rows < 0) return fail(PRISM_ERR_BAD_ARG, "%s: n_seqs must be positive, seq_len and rows not negative", what);
   if (a.cu == nullptr && (long long)a.n * a.len != a.rows)
     return fail(PRISM_ERR_BAD_ARG, "%s: rows must be n_seqs * seq_len without cu_seqlens", what);
@@ -98,6 +101,7 @@ extern "C" int prism_attn_decode(const void* q, const void* k, const void* v, vo
                                  void* scratch, size_t scratch_bytes, void* stream) {
   const char* what = "prism_attn_decode";
   if (n_seqs < 0 || room < 0) return fail(PRISM_ERR_BAD_ARG, "%s: n_seqs and room must not be negative", what);
+  if (room > kMostRows) return fail(PRISM_ERR_UNSUPPORTED, "%s: room for more than %d rows", what, kMostRows);
   if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
     return fail(PRISM_ERR_BAD_ARG, "%s: heads (%d) must be a multiple of kv_heads (%d)", what, heads, kv_heads);
   if (head_dim < 8 || head_dim > 128 || head_dim % 8 != 0)

@@ -219,3 +219,14 @@ def test_c_layer_norm_refuses(built_lib):
     g = lambda dy=P, scratch=P, nbytes=need - 1: L.prism_layer_norm_bwd(dy, None, P, P, P, P, P, P, P, 4, 8, 1, 1, 8, 8, 8, scratch,
                                                                       nbytes, None)
     assert g() == 3 and g(scratch=None) == 3 and g(dy=None) == 1
+
+
+def test_more_rows_than_row_numbers_hold_are_refused(built_lib):
+    """Row numbers rounded up to whole tiles are 32-bit in the kernels."""
+    most = (1 << 31) - 257
+    assert _attn(built_lib, length=most + 1, rows=most + 1) == 2 and _attn(built_lib, cu=P, rows=most + 1) == 2
+    assert _attn(built_lib, length=most, rows=most, ws=128) == 3   # (the last check of all)
+    need = built_lib.prism_attn_decode_scratch_bytes(64)
+    dec = lambda room: built_lib.prism_attn_decode(P, P, P, P, P, 2, room, 4, 2, 64, 1, ctypes.c_float(0.1), (LL * 8)(*(256,) * 8),
+                                                   P, need - 1, None)
+    assert dec(most + 1) == 2 and dec(most) == 3

@@ -184,6 +184,16 @@ def test_many_sequences():
 
 
 @gpu
+def test_many_sequences_take_a_cta_several_searches():
+    """1500 sequences, some empty: every CTA works on several of their tiles and looks for each from where it found the last."""
+    gen = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 40, (1500,), generator=gen).tolist()
+    q, k, v, do = _inputs(lens, 4, 2, 64, torch.bfloat16)
+    _close(_run(q, k, v, do, _cu(lens)), *_exact(q, k, v, do, lens, 0.125))
+    cp.check_device_status()
+
+
+@gpu
 @pytest.mark.parametrize("case", [(5000, 2, 1, 128), (3001, 3, 3, 64)])
 def test_long_sequences(case):
     n, hq, hkv, d = case
