@@ -17,6 +17,7 @@ from . import _lib
 from ._module import _plain_eager, _plain_grad
 
 _MOST_ROWS = (1 << 31) - 257   # (the kernels' row numbers, rounded up to whole tiles, are 32-bit)
+_MOST_SEQUENCES = 1 << 20      # (packed)
 _STRIDES8, _STRIDES9, _STRIDES12 = (ctypes.c_longlong * n for n in (8, 9, 12))
 
 
@@ -66,6 +67,8 @@ def _check_prompt(q, k, v, cu_seqlens) -> None:
     if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2
             or not cu_seqlens.is_contiguous() or cu_seqlens.device != q.device):
         raise ValueError("cu_seqlens must be a contiguous int32 tensor (sequences + 1,) on the device of q")
+    if cu_seqlens.numel() - 1 > _MOST_SEQUENCES:
+        raise ValueError(f"more than {_MOST_SEQUENCES} packed sequences")
 
 
 def _steps(t):
@@ -215,7 +218,7 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
 
     Packed: q ``(rows, heads, head_dim)``, k and v ``(rows, kv_heads, head_dim)`` with ``cu_seqlens``
     ``(sequences + 1,)`` int32 on the same device, sequence i in rows ``cu_seqlens[i]`` up to ``cu_seqlens[i + 1]``
-    (ascending; lengths of zero are allowed; never read by the host).  Rows that belong to no sequence are zeros in the
+    (ascending; lengths of zero are allowed; up to 2^20 sequences; never read by the host).  Rows that belong to no sequence are zeros in the
     output and in the gradients.  Without ``cu_seqlens`` the tensors are one sequence, or, 4D
     ``(batch, rows, heads, head_dim)``, a batch of them.  float16 or bfloat16; ``heads`` a multiple of ``kv_heads``
     (neighbouring query heads share a key head); ``head_dim`` a multiple of 8 up to 128; ``scale`` positive, by default

@@ -43,7 +43,7 @@ __device__ __forceinline__ int attn_clamp(int x, int lo, int hi) { return min(ma
 constexpr int kOwn = 8;
 struct AttnOrder {
   int nt[kOwn];
-  int total, most;   // packed, by levels: all tiles, tiles of the longest sequence
+  int total, most;   // packed: all tiles (by scanning: once they are known), by levels: tiles of the longest sequence
   bool levels;
   int from, before;  // packed, by scanning: where the last search ended, and the tiles before it
 };
@@ -68,7 +68,7 @@ __device__ __forceinline__ AttnOrder attn_order(const AttnRows& r, int bm) {
     sum += o.nt[k];
     top = max(top, o.nt[k]);
   }
-  o.total = __reduce_add_sync(0xffffffffu, sum);
+  o.total = o.levels ? __reduce_add_sync(0xffffffffu, sum) : 0x7fffffff;
   o.most = __reduce_max_sync(0xffffffffu, top);
   return o;
 }
@@ -88,9 +88,8 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, AttnOrder& o, i
   const int lane = threadIdx.x & 31;
   w.tile = -1;
   w.len = w.row = w.batch = 0;
-  int base = 0;
+  int base = o.total;
   if (o.levels) {
-    base = o.total;
     if (idx < o.total) {
       auto above = [&](int level) {
         int c = 0;
@@ -121,7 +120,7 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, AttnOrder& o, i
         left -= c;
       }
     }
-  } else {
+  } else if (idx < o.total) {
     if (idx < o.before) o.from = o.before = 0;
     base = o.before;
     for (int b0 = o.from; b0 < r.n; b0 += 32) {
@@ -148,6 +147,7 @@ __device__ __forceinline__ AttnWork attn_find(const AttnRows& r, AttnOrder& o, i
       }
       base += __shfl_sync(0xffffffffu, incl, 31);
     }
+    if (w.tile < 0) o.total = base;
   }
   w.orow = w.row;
   if (w.tile < 0) {

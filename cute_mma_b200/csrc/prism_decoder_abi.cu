@@ -28,11 +28,13 @@ int num_sms() {   // of the current device; 148 without one
 }
 
 constexpr int kMostRows = 0x7fffffff - 256;   // (row numbers rounded up to whole tiles are ints)
+constexpr int kMostSeqs = 1 << 20;   // packed (looked through while others wait, whose limit is about a second)
 
 AttnStrides strides_at(const long long* s, int i) { return AttnStrides{s[3 * i], s[3 * i + 1], s[3 * i + 2]}; }
 
 int check_attn(const char* what, const AttnArgs& a, const long long* strides, int n_strides) {
   if (a.rows > kMostRows) return fail(PRISM_ERR_UNSUPPORTED, "%s: more than %d rows", what, kMostRows);
+  if (a.cu != nullptr && a.n > kMostSeqs) return fail(PRISM_ERR_UNSUPPORTED, "%s: more than %d packed sequences", what, kMostSeqs);
   if (a.n < 1 || a.len < 0 || a.rows < 0) return fail(PRISM_ERR_BAD_ARG, "%s: n_seqs must be positive, seq_len and rows not negative", what);
   if (a.cu == nullptr && (long long)a.n * a.len != a.rows)
     return fail(PRISM_ERR_BAD_ARG, "%s: rows must be n_seqs * seq_len without cu_seqlens", what);

@@ -226,6 +226,7 @@ def test_more_rows_than_row_numbers_hold_are_refused(built_lib):
     most = (1 << 31) - 257
     assert _attn(built_lib, length=most + 1, rows=most + 1) == 2 and _attn(built_lib, cu=P, rows=most + 1) == 2
     assert _attn(built_lib, length=most, rows=most, ws=128) == 3   # (the last check of all)
+    assert _attn(built_lib, cu=P, n=(1 << 20) + 1, rows=8) == 2 and _attn(built_lib, cu=P, n=1 << 20, rows=8, ws=128) == 3
     need = built_lib.prism_attn_decode_scratch_bytes(64)
     dec = lambda room: built_lib.prism_attn_decode(P, P, P, P, P, 2, room, 4, 2, 64, 1, ctypes.c_float(0.1), (LL * 8)(*(256,) * 8),
                                                    P, need - 1, None)

@@ -194,6 +194,16 @@ def test_many_sequences_take_a_cta_several_searches():
 
 
 @gpu
+def test_a_padded_list_of_offsets():
+    """A few sequences and 100000 empty ones behind them, whose tiles of the grid have nothing to work on."""
+    lens = (130, 1, 0, 300, 40)
+    q, k, v, do = _inputs(lens, 4, 2, 64, torch.bfloat16, seed=9)
+    cu = torch.cat([_cu(lens), torch.full((100000,), sum(lens), dtype=torch.int32, device=DEV)])
+    _close(_run(q, k, v, do, cu), *_exact(q, k, v, do, lens, 0.125))
+    cp.check_device_status()
+
+
+@gpu
 @pytest.mark.parametrize("case", [(5000, 2, 1, 128), (3001, 3, 3, 64)])
 def test_long_sequences(case):
     n, hq, hkv, d = case
