@@ -6,7 +6,9 @@
 // and key heads stand in one line, and every CTA takes an equal stretch of it, whatever the lengths are: no CTA waits for
 // the longest sequence, and a single long one is spread over the whole GPU.  A stretch may begin or end inside a
 // sequence; what a CTA has of such a sequence (maximum, sum, weighted values, fp32) goes to scratch, and a second
-// launch joins the pieces in order: bit-stable.  The lengths are read on the GPU only.
+// launch joins the pieces in order: bit-stable.  The lengths are read on the GPU only.  The join's CTAs stand for stretches,
+// not sequences, which each would look through all lengths (1024 sequences of 256 keys: 311 -> 204 us, 4096 of 128: 2.09 ->
+// 0.59 ms, 64 of 8192: 134 -> 132 us).
 // Measured, bf16, 32 sequences of 4000 keys, 8 key heads of 128 for 32 query heads (525 MB): 87 us, 6.0 TB/s, and 8 us for
 // the join (92 % of the measured copy rate without it).
 //
@@ -38,22 +40,13 @@ __device__ __forceinline__ int decode_len(const DecodeParams& p, int b) {
 __device__ __forceinline__ int decode_tiles(const DecodeParams& p, int b) {
   return (decode_len(p, b) + kTileKeys - 1) / kTileKeys;
 }
-// Tiles of the sequences before `upto` and of all of them, for one key head; by one warp.
-__device__ __forceinline__ void decode_scan(const DecodeParams& p, int upto, long long* before, long long* total) {
-  const int lane = threadIdx.x & 31;
-  long long a = 0, t = 0;
-  for (int b = lane; b < p.n; b += 32) {
-    const int nt = decode_tiles(p, b);
-    t += nt;
-    if (b < upto) a += nt;
-  }
+// Tiles of all sequences, for one key head; by one warp.
+__device__ __forceinline__ long long decode_total(const DecodeParams& p) {
+  long long t = 0;
+  for (int b = threadIdx.x & 31; b < p.n; b += 32) t += decode_tiles(p, b);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, d);
-    t += __shfl_xor_sync(0xffffffffu, t, d);
-  }
-  *before = a;
-  *total = t;
+  for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+  return t;
 }
 
 // A position in the line of tiles.
@@ -74,6 +67,36 @@ struct Cursor {
     } while (nt == 0);
   }
 };
+
+// Where tile `first` of the line is (there is such a tile); by one warp.
+__device__ __forceinline__ Cursor decode_find(const DecodeParams& p, long long first) {
+  const int lane = threadIdx.x & 31, hcs = p.hkv * p.chunks;
+  long long at = 0;
+  Cursor c;
+  c.b = 0;
+  for (int b0 = 0; b0 < p.n; b0 += 32) {
+    const int nt = b0 + lane < p.n ? decode_tiles(p, b0 + lane) : 0;
+    long long incl = nt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, first < (at + incl) * hcs);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      c.b = b0 + l;
+      at += __shfl_sync(0xffffffffu, incl - nt, l);
+      break;
+    }
+    at += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  c.open(p);
+  const long long off = first - at * hcs;
+  c.hc = (int)(off / c.nt);
+  c.t = (int)(off - (long long)c.hc * c.nt);
+  return c;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -117,41 +140,11 @@ __global__ void __launch_bounds__(kWarps * 32, KD <= 4 ? 3 : 2) attn_decode_kern
   extern __shared__ __align__(16) uint8_t dsmem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  long long before, total;
-  decode_scan(p, 0, &before, &total);
-  const int hcs = p.hkv * p.chunks;
-  total *= hcs;
+  const long long total = decode_total(p) * p.hkv * p.chunks;
   const long long share = (total + p.ctas - 1) / p.ctas;
   const long long first = share * blockIdx.x, last = min(first + share, total);
   if (first >= last) return;
-  // where the stretch begins (every warp finds it for itself)
-  Cursor ld;
-  {
-    long long at = 0;
-    int b = 0;
-    for (int b0 = 0; b0 < p.n; b0 += 32) {
-      const int nt = b0 + lane < p.n ? decode_tiles(p, b0 + lane) : 0;
-      long long incl = nt;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, first < (at + incl) * hcs);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        b = b0 + l;
-        at += __shfl_sync(0xffffffffu, incl - nt, l);
-        break;
-      }
-      at += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    ld.b = b;
-    ld.open(p);
-    const long long off = first - at * hcs;
-    ld.hc = (int)(off / ld.nt);
-    ld.t = (int)(off - (long long)ld.hc * ld.nt);
-  }
+  Cursor ld = decode_find(p, first);   // (every warp finds it for itself)
   Cursor cur = ld;
   const int n = (int)(last - first);
   const uint32_t ring = smem_u32(dsmem) + warp * L::kRing;
@@ -364,32 +357,33 @@ __global__ void __launch_bounds__(kWarps * 32, KD <= 4 ? 3 : 2) attn_decode_kern
   }
 }
 
-// Joins the pieces of the heads that more than one CTA worked on, and writes zeros for sequences without keys: a CTA per
-// query head.  First all pieces' maxima and sums, a thread each, which gives their weights; then the weighted values, a
-// quarter of the pieces to a warp.
+// Joins the pieces of the heads that more than one CTA worked on, and writes zeros for sequences without keys.  A CTA for
+// every query head of every stretch, which has work where a head begins in that stretch and does not end in it: however
+// many sequences there are, there are no more of those than stretches.  First all pieces' maxima and sums, a thread each,
+// which gives their weights; then the weighted values, a quarter of the pieces to a warp.
 constexpr int kMostPieces = 1024;   // CTAs of a launch at most
 template <int DT, int KD>
-__global__ void __launch_bounds__(128) attn_decode_join_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(128) attn_decode_join_kernel(const DecodeParams p, int rows) {
   constexpr int kRow = KD * 16 + 2;
   __shared__ float acc[4][KD * 16], weight[kMostPieces], part_m[4], part_l[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / p.hq, head = blockIdx.x - b * p.hq;
-  const int kvh = head / p.group, in_group = head - kvh * p.group;
-  const int hc = kvh * p.chunks + in_group / kHeads, row = in_group % kHeads;
-  long long before, total;
-  decode_scan(p, b, &before, &total);
-  const int hcs = p.hkv * p.chunks, nt = decode_tiles(p, b);
-  uint16_t* dst = p.o + ((long long)b * p.hq + head) * p.dim;
+  for (int b = blockIdx.x; b < p.n; b += gridDim.x)
+    if (decode_len(p, b) == 0)
+      for (int d = threadIdx.x; d < p.hq * p.dim / 8; d += 128)
+        reinterpret_cast<uint4*>(p.o + (long long)b * p.hq * p.dim)[d] = make_uint4(0u, 0u, 0u, 0u);
+  const int c0 = blockIdx.x / rows, row = blockIdx.x - c0 * rows;
+  const long long total = decode_total(p) * p.hkv * p.chunks;
+  const long long share = (total + p.ctas - 1) / p.ctas, first = share * c0, last = first + share;
+  Cursor at;
+  at.t = at.nt = 0;
+  if (last < total) at = decode_find(p, last - 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");   // (every CTA: the launch must not count as done before the first one)
-  if (nt == 0) {
-    for (int d = threadIdx.x; d < p.dim; d += 128) dst[d] = 0;
-    return;
-  }
-  total *= hcs;
-  const long long share = (total + p.ctas - 1) / p.ctas;
-  const long long t0 = before * hcs + (long long)hc * nt, t1 = t0 + nt;
-  const int c0 = (int)(t0 / share), pieces = (int)((t1 - 1) / share) - c0 + 1;
-  if (pieces == 1) return;
+  const long long begin = last - 1 - at.t;
+  if (last >= total || at.t + 1 == at.nt || begin < first) return;
+  const int kvh = at.hc / p.chunks, h0 = (at.hc - kvh * p.chunks) * kHeads;
+  if (h0 + row >= p.group) return;
+  uint16_t* dst = p.o + ((long long)at.b * p.hq + kvh * p.group + h0 + row) * p.dim;
+  const int pieces = (int)((begin + at.nt - 1) / share) - c0 + 1;
   auto piece = [&](int c) { return p.part + (((long long)(c0 + c) * 2 + (c == 0 ? 1 : 0)) * kHeads + row) * kRow; };
   float m = -INFINITY;
   for (int c = threadIdx.x; c < pieces; c += 128) {
@@ -442,7 +436,8 @@ int launch_t(const DecodeParams& p, cudaStream_t stream) {
   kern<<<p.ctas, kWarps * 32, DecodeSmem<KD>::kBytes, stream>>>(p);
   if (int rc = check_launch("decode attention")) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.n * p.hq));
+  const int rows = p.group < kHeads ? p.group : kHeads;
+  cfg.gridDim = dim3((unsigned)(p.ctas * rows));
   cfg.blockDim = dim3(128);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -450,7 +445,7 @@ int launch_t(const DecodeParams& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<DT, KD>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<DT, KD>, p, rows);
   if (e != cudaSuccess) return fail(PRISM_ERR_CUDA, "decode attention: launch failed: %s", cudaGetErrorString(e));
   return check_launch("decode attention join");
 }

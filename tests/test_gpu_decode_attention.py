@@ -51,6 +51,21 @@ def test_lengths_and_heads(lens, heads, dt):
 
 
 @gpu
+@pytest.mark.parametrize("heads", [(6, 2, 64), (34, 1, 128)])
+def test_more_sequences_than_ctas(heads):
+    """Many short sequences, empty ones among them, and a long one that several CTAs share."""
+    hq, hkv, d = heads
+    gen = torch.Generator().manual_seed(hq)
+    lens = torch.randint(0, 200, (1200,), generator=gen).tolist()
+    lens[::17] = [0] * len(lens[::17])
+    lens[600] = 3000
+    q, k, v = _inputs(len(lens), 3000, hq, hkv, d, torch.bfloat16, seed=d)
+    o = cp.decode_attention(q, k, v, torch.tensor(lens, device=DEV, dtype=torch.int32))
+    _check(o, q, k, v, lens, d ** -0.5)
+    assert torch.equal(o, cp.decode_attention(q, k, v, torch.tensor(lens, device=DEV, dtype=torch.int32)))
+
+
+@gpu
 @pytest.mark.parametrize("d", [8, 16, 24, 40, 56, 80, 96, 104, 112, 120])
 def test_head_dims(d):
     lens = (300, 33)
