@@ -134,6 +134,13 @@ struct DecodeSmem {
   static constexpr int kBytes = kWarps * kRing + kJoin;
 };
 
+// Exponents of P are raised by this, which the sums carry as well, so that it is gone from the quotient.  fp16 ends at 2^-24:
+// with a largest P of 1 many keys that weigh little are lost from the values' product but not from the sum (4099 keys, one of
+// them 17 nats above the others: what the others add up to was 1.5 % off); with 2^15 its whole range is used.  bf16 has fp32's
+// exponents.
+template <int DT>
+__device__ __forceinline__ constexpr float decode_lift() { return DT == DT_F16 ? 15.f : 0.f; }
+
 template <int DT, int KD>
 __global__ void __launch_bounds__(kWarps * 32, KD <= 4 ? 3 : 2) attn_decode_kernel(const DecodeParams p) {
   using L = DecodeSmem<KD>;
@@ -249,7 +256,7 @@ __global__ void __launch_bounds__(kWarps * 32, KD <= 4 ? 3 : 2) attn_decode_kern
       const float base = mx == -INFINITY ? 0.f : mx;
       const float f = f2[h] = ex2((m[h] - base) * p.c);
       m[h] = mx;
-      const float neg = -base * p.c;
+      const float neg = fmaf(-base, p.c, decode_lift<DT>());
       const float e0 = ex2(fmaf(s[0][2 * h], p.c, neg)), e1 = ex2(fmaf(s[0][2 * h + 1], p.c, neg));
       const float e2 = ex2(fmaf(s[1][2 * h], p.c, neg)), e3 = ex2(fmaf(s[1][2 * h + 1], p.c, neg));
       l[h] = l[h] * f + ((e0 + e1) + (e2 + e3));

@@ -1,0 +1,48 @@
+"""Weights and gradients that 16-bit floats of 5 exponent bits can only hold if the kernels use all of their range: many keys
+that weigh little each, and small output gradients over thousands of keys."""
+import math
+
+import pytest
+import torch
+
+import cute_mma_b200 as cp
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -11   # half a step of fp16
+
+
+def _one_loud_key(n, hkv, d, at, seed=0):
+    """Scores (scale 1) of one key 17 nats above a spread of a half; the loud key's values are zeros, so that results are made
+    of the others alone.  q: one head for every key head."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    k = torch.randn(n, hkv, d, device=DEV, generator=gen).half()
+    k[..., 0] = (0.5 * torch.randn(n, hkv, device=DEV, generator=gen)).half()
+    k[at, :, 0] = 17.0
+    v = (1 + torch.randn(n, hkv, d, device=DEV, generator=gen)).half()
+    v[at] = 0
+    q = torch.zeros(hkv, d, device=DEV, dtype=torch.float16)
+    q[:, 0] = 1
+    return q, k, v
+
+
+def _exponent_error(d, q, k, scale):
+    """Twice what d + 8 roundings of fp32 leave of a score, and 2^-20 for exponentials and sums."""
+    return 2 * (d + 8) * 2.0 ** -24 * scale * float((q.double().abs()[:, None] * k.double().abs().transpose(0, 1)).sum(-1).max()) + 2.0 ** -20
+
+
+@gpu
+@pytest.mark.parametrize("case", [(100003, 1, 2, 64, 7), (4099, 700, 2, 64, 0), (2500, 900, 1, 128, 17), (3000, 1000, 3, 24, 40)])
+def test_decode_keys_that_weigh_little(case):
+    """|o - o64| <= (u + e) sum P |v| + u |o|, and what fp16 with a largest weight of 2^15 rounds away below its normal
+    numbers: 2^-25 of 2^-15 of the largest weight, a key.  Many sequences (of one cache) leave whole ones to a CTA."""
+    n, b, hkv, d, at = case
+    q, k, v = _one_loud_key(n, hkv, d, at, seed=d)
+    lengths = torch.full((b,), n, device=DEV, dtype=torch.int32)
+    o = cp.decode_attention(q.expand(b, hkv, d), k.expand(b, n, hkv, d), v.expand(b, n, hkv, d), lengths, scale=1.0).double()
+    P = torch.softmax(torch.einsum("hd,jhd->hj", q.double(), k.double()), -1)
+    want = torch.einsum("hj,jhd->hd", P, v.double())
+    e = _exponent_error(d, q, k, 1.0)
+    tol = (U + e) * torch.einsum("hj,jhd->hd", P, v.double().abs()) + U * want.abs()
+    tol += 2.0 ** -40 * P.amax(-1, keepdim=True) * v.double().abs().sum(0) + 2.0 ** -25
+    assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
