@@ -4,6 +4,8 @@
 //   S = Q K^T (tcgen05, fp32 in TMEM) -> p = 2^(c s - c m) (registers, one row a thread) -> 16 bits, into TMEM
 //   -> O += P V (tcgen05, P from TMEM);  O and l are rescaled only when a row's maximum has grown by more than 2^8
 // (every p stays below 2^8, which costs neither 16-bit type any of its digits); the end divides by l.
+// fp16 ends at 2^-24, where many keys that weigh little would be lost from P V but not from l: there every p, and so l and O,
+// carries a factor of 2^7 more (fwd_lift), up to 2^15 of the type's 2^16.
 // A CTA works on two 128-row tiles at a time with a warpgroup each (two heads of a group, whose keys are the same, or 256
 // rows of one head), so that the tensor core has the other tile's products while a warpgroup is in its exponentials.
 // P is handed over in two pieces: the first one's product runs beside the second one's exponentials.  Keys and values pass
@@ -24,7 +26,7 @@ namespace {
 struct FwdParams {
   AttnRows rows;
   uint16_t* o;     // rows x heads x dim
-  float* lse;      // heads x rows, c m + log2 l per row, or null
+  float* lse;      // heads x rows, c m + log2 of the sum per row, or null
   uint8_t* low;    // rows x heads x dim, what o's rounding took (e5m2), or null
   const uint16_t* v;   // as the tensor map has it, for the rows of infinities and NaN
   AttnStrides sv;
@@ -42,6 +44,9 @@ constexpr int kThreads = 384, kSoftmaxRegs = 208, kOtherRegs = 88;
 // Blocks of keys that are looked through before their product (the tiles' own rows) in turn: at most as many are under way
 // as the ring holds value tiles.
 constexpr int kChecks = 8;
+
+template <int DT>
+__device__ __forceinline__ constexpr float fwd_lift() { return DT == DT_F16 ? 7.f : 0.f; }
 
 template <int DH>
 struct FwdSmem {
@@ -396,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float2 c2 = both(p.c), n2 = both(m == -INFINITY ? 0.f : -m * p.c);
+        const float2 c2 = both(p.c), n2 = both(fmaf(m == -INFINITY ? 0.f : -m, p.c, fwd_lift<DT>()));
         float2 sum0 = both(0.f), sum1 = both(0.f);
         // Wide heads: the exponentials of the two warps of a quarter SM take turns, so that one tile's run beside the
         // other's products (8192 rows, 16 heads of 128: 288 -> 244 us).  Where S does not wait for P V there is nothing to
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();   // (its row was stored by the lanes beside it)
       if (*static_cast<volatile int*>(&bars.unbounded) && mine)
         attn_add_unbounded<DT>(p, w, (tl.n[0] - 1) * kAttnTile, row, head / p.group, p.o + at + lane * step);
-      if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + lg2(l);
+      if (mine && p.lse != nullptr) p.lse[(long long)head * p.rows.rows + w.orow + row] = m * p.c + (lg2(l) - fwd_lift<DT>());
     }
   }
   if (!ok && lane == 0) atomicExch(p.err, PRISM_ERR_DEVICE_WAIT);

@@ -46,3 +46,19 @@ def test_decode_keys_that_weigh_little(case):
     tol = (U + e) * torch.einsum("hj,jhd->hd", P, v.double().abs()) + U * want.abs()
     tol += 2.0 ** -40 * P.amax(-1, keepdim=True) * v.double().abs().sum(0) + 2.0 ** -25
     assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("case", [(4099, 2, 64, 0), (3000, 1, 128, 17), (2500, 3, 80, 1)])
+def test_prompt_keys_that_weigh_little(case):
+    """As above, with a largest weight of 2^7 to 2^15 (its reference is the row's maximum or one 2^8 below)."""
+    n, hkv, d, at = case
+    q, k, v = _one_loud_key(n, hkv, d, at, seed=d)
+    o = cp.causal_attention(q.expand(n, hkv, d), k, v, scale=1.0).double()
+    s = torch.einsum("hd,jhd->hj", q.double(), k.double())[:, None].expand(hkv, n, n)
+    P = torch.softmax(s.masked_fill(~torch.ones(n, n, device=DEV, dtype=torch.bool).tril(), -math.inf), -1)
+    want = torch.einsum("hij,jhd->ihd", P, v.double())
+    e = _exponent_error(d, q, k, 1.0)
+    tol = (U + e) * torch.einsum("hij,jhd->ihd", P, v.double().abs()) + U * want.abs()
+    tol += 2.0 ** -32 * P.amax(-1).T[..., None] * v.double().abs().cumsum(0) + 2.0 ** -25
+    assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
