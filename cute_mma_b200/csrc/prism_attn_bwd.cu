@@ -6,6 +6,9 @@
 // to clear and convert, the same bits every run.  A key tile walks through all query heads of its group, so that the
 // gradients of shared heads are sums in TMEM as well.
 //
+// fp16 ends at 2^-24, and P of a row of n keys is about 1/n: P^T carries a factor of 2^15 there (bwd_lift), which dv's store
+// takes out again and dS does not get.
+//
 // Measured, bf16, one sequence of 8192 rows, 16 heads: of 128, dk and dv 460 us (tensor pipe 57 % busy: bound by the chain
 // S -> P -> dS -> dk of a tile, whose two accumulators leave no TMEM for a second tile), dq 280 us (86 %: bound by the
 // tensor pipe); of 64, 335 and 208 us (38 and 46 %: bound by the arithmetic between the products).  delta takes 20 us.
@@ -29,6 +32,9 @@ struct BwdParams {
 // Two warpgroups of arithmetic, and one of the loading warp, the issuing warps and (dk, dv) the warp of the row statistics.
 //  256 x 208 + 128 x 88 registers = 384 x 168, what the block is launched with.
 constexpr int kThreads = 384, kMathRegs = 208, kOtherRegs = 88;
+
+template <int DT>
+__device__ __forceinline__ constexpr float bwd_lift() { return DT == DT_F16 ? 15.f : 0.f; }
 
 // ---------------------------------------------------------------------------------------------------- delta
 // Sixteen lanes a row of a head: 16-byte pieces of o and do, and 8 bytes of what o's rounding took.  An error of delta is
@@ -109,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DkvBars bars;
   __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated
+  __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated; P's factor in the one, its inverse in the other
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 
@@ -202,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the row statistics; and a sequence's last tiles are cleaned behind its end before any product reads them
       Ring rq(L::kQ), rd(L::kDo);
       uint32_t cnt = 0, cleaned = 0;
+      const float drop = pow2i(-(int)bwd_lift<DT>());
       while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
         const int nq = q_tiles(w), n = nq * p.group;
         int head = kvh * p.group, i = 0;
@@ -211,8 +218,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int row = (w.tile + i) * kAttnTile + e * 32 + lane;
-            a[e] = row < w.len ? -__ldg(p.lse + at + row) : -INFINITY;
-            b[e] = row < w.len ? -__ldg(p.delta + at + row) : 0.f;
+            a[e] = row < w.len ? bwd_lift<DT>() - __ldg(p.lse + at + row) : -INFINITY;
+            b[e] = row < w.len ? -__ldg(p.delta + at + row) * drop : 0.f;
           }
           const int valid = w.len - (w.tile + i) * kAttnTile;
           if (valid < kAttnTile) {
@@ -332,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t dp_addr = tmem + lanes + kDp + half * 64;
     const int key = (warp & 3) * 32 + lane;
-    const float2 c2 = both(p.c);
+    const float2 c2 = both(p.c), drop2 = both(pow2i(-(int)bwd_lift<DT>()));
     const float4* lse = reinterpret_cast<const float4*>(st_lse + half * 64);
     const float4* del = reinterpret_cast<const float4*>(st_delta + half * 64);
     uint32_t cnt = 0, used = 0;
@@ -389,8 +396,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 z = del[(c * 32 + e) >> 2];
-            float2 x = add2(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), make_float2(z.x, z.y));
-            float2 y = add2(make_float2(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), make_float2(z.z, z.w));
+            float2 x = make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
+            float2 y = make_float2(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3]));
+            x = DT == DT_F16 ? fma2(x, drop2, make_float2(z.x, z.y)) : add2(x, make_float2(z.x, z.y));
+            y = DT == DT_F16 ? fma2(y, drop2, make_float2(z.z, z.w)) : add2(y, make_float2(z.z, z.w));
             x = mul2(x, make_float2(__uint_as_float(s[c * 32 + e]), __uint_as_float(s[c * 32 + e + 1])));
             y = mul2(y, make_float2(__uint_as_float(s[c * 32 + e + 2]), __uint_as_float(s[c * 32 + e + 3])));
             dp[e] = __float_as_uint(x.x); dp[e + 1] = __float_as_uint(x.y);
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const int row0 = w.tile * kAttnTile + key - lane;
       const long long at = ((w.orow + row0) * p.hkv + kvh) * p.dim, step = (long long)p.hkv * p.dim;
-      if (half == 0) attn_store_rows<DT, DH, false>(tmem + lanes + kDv, 1.f, p.dv + at, nullptr, step, p.dim, w.len - row0);
+      if (half == 0) attn_store_rows<DT, DH, false>(tmem + lanes + kDv, drop2.x, p.dv + at, nullptr, step, p.dim, w.len - row0);
       else attn_store_rows<DT, DH, false>(tmem + lanes + kDk, p.scale, p.dk + at, nullptr, step, p.dim, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();

@@ -62,3 +62,31 @@ def test_prompt_keys_that_weigh_little(case):
     tol = (U + e) * torch.einsum("hij,jhd->ihd", P, v.double().abs()) + U * want.abs()
     tol += 2.0 ** -32 * P.amax(-1).T[..., None] * v.double().abs().cumsum(0) + 2.0 ** -25
     assert ((o - want).abs() <= tol).all(), float(((o - want).abs() / tol).max())
+
+
+def _causal(n):
+    return torch.ones(n, n, device=DEV, dtype=torch.bool).tril()
+
+
+def _gradients(q, k, v, do, scale):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = torch.autograd.grad(cp.causal_attention(*leaves, scale=scale), leaves, do)
+    cp.check_device_status()
+    return [t.double() for t in out]
+
+
+@gpu
+@pytest.mark.parametrize("case", [(4099, 64, 0), (3000, 128, 17), (2500, 80, 1)])
+def test_value_gradients_of_keys_that_weigh_little(case):
+    """|dv - dv64| <= (u + e) sum_i P |do| + u |dv|, and 2^-25 of 2^-15 a row: P has a factor of 2^15."""
+    n, d, at = case
+    q, k, v = _one_loud_key(n, 1, d, at, seed=d)
+    do = (1 + torch.randn(n, 1, d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n))).half()
+    dv = _gradients(q.expand(n, 1, d), k, v, do, 1.0)[2][:, 0]
+    s = (k[:, 0].double() @ q[0].double()).expand(n, n)
+    P = torch.softmax(s.masked_fill(~_causal(n), -math.inf), -1)
+    G = do[:, 0].double()
+    want = P.T @ G
+    e = _exponent_error(d, q, k, 1.0)
+    tol = (U + e) * (P.T @ G.abs()) + U * want.abs() + 2.0 ** -40 * G.abs().flip(0).cumsum(0).flip(0) + 2.0 ** -25
+    assert ((dv - want).abs() <= tol).all(), float(((dv - want).abs() / tol).max())
