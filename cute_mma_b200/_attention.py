@@ -138,12 +138,12 @@ def _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, scale, need_dq=True, n
     v, sv = _tma_rows(v)
     n, length = _sequences(q, cu_seqlens)
     with F._device_scope(q.device):
-        delta = lse.new_empty(lse.shape)
+        delta = lse.new_empty(lse.numel() + 2)   # (and the largest norms of d_o and v behind it)
         ws = F._workspace.get(q.device, 256)
-        _lib.check(_lib.lib().prism_attn_bwd(
+        _lib.check(_lib.lib().prism_attn_bwd_scaled(
             d_o.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), F._ptr(low), F._ptr(dq),
-            F._ptr(dk), F._ptr(dv), delta.data_ptr(), F._ptr(cu_seqlens), n, length, rows, hq, k.shape[-2], d, F._DTYPES[q.dtype],
-            scale, _STRIDES12(*sq, *sk, *sv, *sdo), ws.data_ptr(), ws.numel(), F._raw_stream(q.device)))
+            F._ptr(dk), F._ptr(dv), delta.data_ptr(), delta.data_ptr() + 4 * lse.numel(), F._ptr(cu_seqlens), n, length, rows,
+            hq, k.shape[-2], d, F._DTYPES[q.dtype], scale, _STRIDES12(*sq, *sk, *sv, *sdo), ws.data_ptr(), ws.numel(), F._raw_stream(q.device)))
     return dq, dk, dv
 
 

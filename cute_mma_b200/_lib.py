@@ -31,7 +31,7 @@ NVCC_FLAGS = [
 EXPORTS = [
     "prism_fwd", "prism_fwd_dropout", "prism_fwd_noalloc", "prism_bwd_dadr", "prism_bwd_db", "prism_dbias", "prism_fold_weight", "prism_cayley", "prism_cayley_bwd", "prism_peer_reduce",
     "prism_bwd_dadr_mask", "prism_bwd_db_mask", "prism_dropout_mask_bytes", "prism_shuffle_cols", "prism_shuffle_fold_r", "prism_shuffle_unfold_r", "prism_workspace_bytes",
-    "prism_status", "prism_attn_fwd", "prism_attn_bwd", "prism_attn_decode", "prism_attn_decode_scratch_bytes",
+    "prism_status", "prism_attn_fwd", "prism_attn_bwd", "prism_attn_bwd_scaled", "prism_attn_decode", "prism_attn_decode_scratch_bytes",
     "prism_layer_norm", "prism_layer_norm_bwd", "prism_layer_norm_scratch_bytes",
     "prism_last_error_string", "prism_abi_version", "prism_launch_count",
 ]
@@ -164,6 +164,8 @@ def lib() -> ctypes.CDLL:
             L.prism_attn_fwd.argtypes = [vp] * 7 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_attn_bwd.restype = i
             L.prism_attn_bwd.argtypes = [vp] * 12 + [i] * 7 + [fl, llp, vp, sz, vp]
+            L.prism_attn_bwd_scaled.restype = i
+            L.prism_attn_bwd_scaled.argtypes = [vp] * 13 + [i] * 7 + [fl, llp, vp, sz, vp]
             L.prism_attn_decode_scratch_bytes.restype = sz
             L.prism_attn_decode_scratch_bytes.argtypes = [i]
             L.prism_attn_decode.restype = i

@@ -7,7 +7,9 @@
 // gradients of shared heads are sums in TMEM as well.
 //
 // fp16 ends at 2^-24, and P of a row of n keys is about 1/n: P^T carries a factor of 2^15 there (bwd_lift), which dv's store
-// takes out again and dS does not get.
+// takes out again and dS does not get.  dS has a factor of its own, 2^e with |dS| 2^e <= 2^15: |dS_ij| <= |do_i| |v_j - o_i|
+// <= 2 max |do| max |v| (o_i lies among the values), and the delta pass, which reads do anyway, takes both maxima.  Unscaled,
+// 8192 keys and do of 1e-3 gave dq and dk 1 % off, and do of 1e4 gave infinities.
 //
 // Measured, bf16, one sequence of 8192 rows, 16 heads: of 128, dk and dv 460 us (tensor pipe 57 % busy: bound by the chain
 // S -> P -> dS -> dk of a tile, whose two accumulators leave no TMEM for a second tile), dq 280 us (86 %: bound by the
@@ -26,6 +28,7 @@ struct BwdParams {
   const float *lse, *delta;   // heads x rows
   int hq, hkv, group, dim;
   float c, scale;             // scale * log2 e, scale
+  const float* norms;         // fp16: largest squares of the norms of do's and of v's rows (null: dS as it is)
   int* err;
 };
 
@@ -36,51 +39,122 @@ constexpr int kThreads = 384, kMathRegs = 208, kOtherRegs = 88;
 template <int DT>
 __device__ __forceinline__ constexpr float bwd_lift() { return DT == DT_F16 ? 15.f : 0.f; }
 
+// e of dS's factor 2^e.  Norms of zero leave nothing to scale; 40 is as good as any.
+template <int DT>
+__device__ __forceinline__ int ds_exponent(const float* norms) {
+  if (DT != DT_F16 || norms == nullptr) return 0;
+  const float e = floorf(13.99f - 0.5f * (lg2(__ldg(norms)) + lg2(__ldg(norms + 1))));
+  return (int)fminf(fmaxf(e, -40.f), 40.f);
+}
+
 // ---------------------------------------------------------------------------------------------------- delta
-// Sixteen lanes a row of a head: 16-byte pieces of o and do, and 8 bytes of what o's rounding took.  An error of delta is
-// one of every dS of its row with the same sign, which no sum over the keys averages out: with o as rounded alone dq was
-// 0.0025 off (relative norm, 1024 rows, heads of 64, bf16), with the rest 0.0024, of which 0.0023 is the rounding of dS.
+// LANES lanes (8 for heads of up to 64, 16 for wider ones) have 16-byte pieces of a row's o and do, and 8 bytes of what o's
+// rounding took, for kDeltaHeads heads one after the other.  An error of delta is one of every dS of its row with the same sign,
+// which no sum over the keys averages out: with o as rounded alone dq was 0.0025 off (relative norm, 1024 rows, heads of 64,
+// bf16), with the rest 0.0024, of which 0.0023 is the rounding of dS.  16 x 1024 rows, 12 heads of 64: 25 us with a division for
+// every 16 bytes; now, with norms, 19 us (and one of the clearing before it).
+constexpr int kDeltaHeads = 4;
 struct DeltaParams {
   const uint16_t *o, *d_o;
   const uint8_t* low;
   AttnStrides sdo;
   float* delta;
-  int heads, dim, len;   // len: rows per batch entry
-  long long rows;
+  int heads, dim, len, rows;   // len: rows per batch entry
+  unsigned groups, all_groups;   // of heads: of o, and of o and (NORMS) v behind them
+  const uint16_t* v;             // NORMS
+  AttnStrides sv;
+  const int* cu;
+  int n, kv_heads;
+  float* norms;
 };
-template <int DT>
+
+// The largest of a block's squared norms to *most.
+__device__ __forceinline__ void attn_largest(float sq, float* most) {
+  __shared__ float red[8];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sq = fmaxf(sq, __shfl_xor_sync(0xffffffffu, sq, d));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sq;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) sq = fmaxf(sq, red[i]);
+  // (bits of floats that are not negative are in their order; a maximum does not depend on the order that it is taken in)
+  if (sq > __ldcg(most)) atomicMax(reinterpret_cast<int*>(most), __float_as_int(sq));
+}
+
+template <int DT, bool NORMS, int LANES>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const DeltaParams p) {
-  const long long unit = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int piece = threadIdx.x & 15;
-  float sum = 0.f;
-  const long long row = unit / p.heads;
-  const int head = (int)(unit - row * p.heads);
-  if (row < p.rows && piece * 8 < p.dim) {
-    const long long b = row / p.len;
-    const uint4 x = *reinterpret_cast<const uint4*>(p.o + unit * p.dim + piece * 8);
-    const uint4 y = *reinterpret_cast<const uint4*>(p.d_o + b * p.sdo.batch + (row - b * p.len) * p.sdo.row +
-                                                    head * p.sdo.head + piece * 8);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  const int piece = threadIdx.x & (LANES - 1);
+  const unsigned block = blockIdx.x / p.all_groups;
+  unsigned group = blockIdx.x - block * p.all_groups;
+  const int row = (int)(block * (256 / LANES) + threadIdx.x / LANES);
+  const bool values = NORMS && group >= p.groups;
+  if (values) group -= p.groups;
+  const int heads = values ? p.kv_heads : p.heads, head0 = (int)group * kDeltaHeads;
+  const bool there = row < p.rows, inside = there && piece * 8 < p.dim;
+  const int b = there ? row / p.len : 0;
+  const AttnStrides& st = values ? p.sv : p.sdo;
+  const uint16_t* y0 = (values ? p.v : p.d_o) + b * st.batch + (long long)(row - b * p.len) * st.row + piece * 8;
+  const long long at0 = (long long)row * p.heads * p.dim + piece * 8;
+  uint4 x[kDeltaHeads], y[kDeltaHeads];
+  uint2 z[kDeltaHeads];
+#pragma unroll
+  for (int h = 0; h < kDeltaHeads; ++h) {
+    const bool live = inside && head0 + h < heads;
+    x[h] = y[h] = make_uint4(0u, 0u, 0u, 0u);
+    z[h] = make_uint2(0u, 0u);
+    if (!live) continue;
+    y[h] = *reinterpret_cast<const uint4*>(y0 + (head0 + h) * st.head);
+    if (values) continue;
+    const long long at = at0 + (long long)(head0 + h) * p.dim;
+    x[h] = *reinterpret_cast<const uint4*>(p.o + at);
+    if (p.low != nullptr) z[h] = *reinterpret_cast<const uint2*>(p.low + at);
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int h = 0; h < kDeltaHeads; ++h) {
+    const uint32_t xs[4] = {x[h].x, x[h].y, x[h].z, x[h].w}, ys[4] = {y[h].x, y[h].y, y[h].z, y[h].w};
+    float sum = 0.f, sq = 0.f, rest = 0.f, f[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 a = Elem<DT>::unpack(xs[e]), b2 = Elem<DT>::unpack(ys[e]);
-      sum = fmaf(a.x, b2.x, fmaf(a.y, b2.y, sum));
+      const float2 a = Elem<DT>::unpack(xs[e]), g = Elem<DT>::unpack(ys[e]);
+      sum = fmaf(a.x, g.x, fmaf(a.y, g.y, sum));
+      if ((e & 1) == 0) unpack_e5m2(e == 0 ? z[h].x : z[h].y, f);
+      rest = fmaf(f[(e & 1) * 2], g.x, fmaf(f[(e & 1) * 2 + 1], g.y, rest));
+      if (NORMS) sq = fmaf(g.x, g.x, fmaf(g.y, g.y, sq));
     }
-    if (p.low != nullptr) {
-      const uint2 z = *reinterpret_cast<const uint2*>(p.low + unit * p.dim + piece * 8);
-      float f[4], rest = 0.f;
+    if (p.low != nullptr) sum = fmaf(rest, 1.f / low_scale<DT>(), sum);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if ((e & 1) == 0) unpack_e5m2(e == 0 ? z.x : z.y, f);
-        const float2 b2 = Elem<DT>::unpack(ys[e]);
-        rest = fmaf(f[(e & 1) * 2], b2.x, fmaf(f[(e & 1) * 2 + 1], b2.y, rest));
-      }
-      sum = fmaf(rest, 1.f / low_scale<DT>(), sum);
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (NORMS) sq += __shfl_xor_sync(0xffffffffu, sq, d);
     }
+    if (!values && there && piece == 0 && head0 + h < heads) p.delta[(long long)(head0 + h) * p.rows + row] = sum;
+    // (a row that is not finite does not count: what it gives is not either)
+    if (NORMS && isfinite(sq)) most = fmaxf(most, sq);
   }
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (row < p.rows && piece == 0) p.delta[head * p.rows + row] = sum;
+  if constexpr (NORMS) {
+    // rows of no sequence do not count
+    const int front = p.cu == nullptr ? 0 : attn_clamp(__ldg(p.cu), 0, p.rows);
+    const int end = p.cu == nullptr ? p.rows : attn_clamp(__ldg(p.cu + p.n), front, p.rows);
+    attn_largest(row >= front && row < end ? most : 0.f, p.norms + values);
+  }
+}
+
+template <int DT, bool NORMS>
+int launch_delta(DeltaParams d, cudaStream_t stream) {
+  const int lanes = d.dim <= 64 ? 8 : 16;
+  d.groups = ((unsigned)d.heads + kDeltaHeads - 1) / kDeltaHeads;
+  d.all_groups = d.groups + (NORMS ? ((unsigned)d.kv_heads + kDeltaHeads - 1) / kDeltaHeads : 0u);
+  const long long blocks = ((long long)d.rows + 256 / lanes - 1) / (256 / lanes) * d.all_groups;
+  if (blocks > 0x7fffffffll) return fail(PRISM_ERR_UNSUPPORTED, "attention: more than 2^31 blocks of rows and heads");
+  if (NORMS) {
+    const cudaError_t e = cudaMemsetAsync(d.norms, 0, 2 * sizeof(float), stream);
+    if (e != cudaSuccess) return fail(PRISM_ERR_CUDA, "causal attention delta: %s", cudaGetErrorString(e));
+  }
+  if (lanes == 8) attn_delta_kernel<DT, NORMS, 8><<<(unsigned)blocks, 256, 0, stream>>>(d);
+  else attn_delta_kernel<DT, NORMS, 16><<<(unsigned)blocks, 256, 0, stream>>>(d);
+  return check_launch("causal attention delta");
 }
 
 // ---------------------------------------------------------------------------------------------------- dk, dv
@@ -115,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DkvBars bars;
   __shared__ AttnSched sched;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated; P's factor in the one, its inverse in the other
+  __shared__ __align__(16) float st_lse[kAttnTile], st_delta[kAttnTile];   // negated; with P's factor, and with what dS's is beyond it
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
 
@@ -208,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the row statistics; and a sequence's last tiles are cleaned behind its end before any product reads them
       Ring rq(L::kQ), rd(L::kDo);
       uint32_t cnt = 0, cleaned = 0;
-      const float drop = pow2i(-(int)bwd_lift<DT>());
+      const float drop = pow2i(ds_exponent<DT>(p.norms) - (int)bwd_lift<DT>());
       while (ok && attn_next(sched, rw, &w, &kvh, &ok)) {
         const int nq = q_tiles(w), n = nq * p.group;
         int head = kvh * p.group, i = 0;
@@ -339,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t dp_addr = tmem + lanes + kDp + half * 64;
     const int key = (warp & 3) * 32 + lane;
-    const float2 c2 = both(p.c), drop2 = both(pow2i(-(int)bwd_lift<DT>()));
+    const int raised = ds_exponent<DT>(p.norms);
+    const float2 c2 = both(p.c), drop2 = both(pow2i(raised - (int)bwd_lift<DT>()));
     const float4* lse = reinterpret_cast<const float4*>(st_lse + half * 64);
     const float4* del = reinterpret_cast<const float4*>(st_delta + half * 64);
     uint32_t cnt = 0, used = 0;
@@ -429,8 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const int row0 = w.tile * kAttnTile + key - lane;
       const long long at = ((w.orow + row0) * p.hkv + kvh) * p.dim, step = (long long)p.hkv * p.dim;
-      if (half == 0) attn_store_rows<DT, DH, false>(tmem + lanes + kDv, drop2.x, p.dv + at, nullptr, step, p.dim, w.len - row0);
-      else attn_store_rows<DT, DH, false>(tmem + lanes + kDk, p.scale, p.dk + at, nullptr, step, p.dim, w.len - row0);
+      if (half == 0) attn_store_rows<DT, DH, false>(tmem + lanes + kDv, pow2i(-(int)bwd_lift<DT>()), p.dv + at, nullptr, step, p.dim, w.len - row0);
+      else attn_store_rows<DT, DH, false>(tmem + lanes + kDk, p.scale * pow2i(-raised), p.dk + at, nullptr, step, p.dim, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.acc_empty);
@@ -613,12 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lanes + half * 64;
     const int r = (warp & 3) * 32 + lane;
     const float2 c2 = both(p.c);
+    const int raised = ds_exponent<DT>(p.norms);
     uint32_t cnt = 0, used = 0;
     while (ok && attn_next(sched, rw, &w, &head, &ok)) {
       const int n = w.tile + 1, row = w.tile * kAttnTile + r;
       const bool mine = row < w.len;
       const long long at = (long long)head * p.rows.rows + w.orow + row;
-      const float2 n2 = both(mine ? -__ldg(p.lse + at) : -INFINITY), d2 = both(mine ? -__ldg(p.delta + at) : 0.f);
+      const float2 n2 = both(mine ? (float)raised - __ldg(p.lse + at) : -INFINITY), d2 = both(mine ? -__ldg(p.delta + at) : 0.f);
       for (int j = 0; j < n; ++j, ++cnt) {
         if (!warp_wait(&bars.s_full, cnt & 1)) { ok = false; break; }
         tc_fence_after_sync();
@@ -675,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after_sync();
       const int row0 = row - lane, part = half * (DH / 2);   // (each warpgroup half of the features)
       if (part < p.dim)
-        attn_store_rows<DT, DH / 2, false>(tmem + lanes + kDq + part, p.scale, p.dq + ((w.orow + row0) * p.hq + head) * p.dim + part,
+        attn_store_rows<DT, DH / 2, false>(tmem + lanes + kDq + part, p.scale * pow2i(-raised), p.dq + ((w.orow + row0) * p.hq + head) * p.dim + part,
                                            nullptr, (long long)p.hq * p.dim, p.dim - part, w.len - row0);
       tc_fence_before_sync();
       __syncwarp();
@@ -730,16 +806,20 @@ int launch_attn_bwd(const AttnArgs& a) {
   d.delta = a.delta;
   d.heads = a.hq; d.dim = a.dim; d.rows = a.rows;
   d.len = a.cu == nullptr ? a.len : a.rows;
-  const long long blocks = ((long long)a.rows * a.hq + 15) / 16;
-  if (blocks > 0x7fffffffll) return fail(PRISM_ERR_UNSUPPORTED, "attention: more than 2^35 rows");
-  if (a.dtype == DT_BF16) attn_delta_kernel<DT_BF16><<<(unsigned)blocks, 256, 0, a.stream>>>(d);
-  else attn_delta_kernel<DT_F16><<<(unsigned)blocks, 256, 0, a.stream>>>(d);
-  if (int rc = check_launch("causal attention delta")) return rc;
+  d.v = static_cast<const uint16_t*>(a.v); d.sv = a.sv;
+  d.cu = a.cu; d.n = a.n; d.kv_heads = a.hkv;
+  d.norms = a.dtype == DT_F16 ? a.norms : nullptr;
+  int rc;
+  if (a.dtype == DT_BF16) rc = launch_delta<DT_BF16, false>(d, a.stream);
+  else if (d.norms == nullptr) rc = launch_delta<DT_F16, false>(d, a.stream);
+  else rc = launch_delta<DT_F16, true>(d, a.stream);
+  if (rc) return rc;
   BwdParams p;
   p.dq = static_cast<uint16_t*>(a.dq); p.dk = static_cast<uint16_t*>(a.dk); p.dv = static_cast<uint16_t*>(a.dv);
   p.lse = a.lse; p.delta = a.delta;
   p.hq = a.hq; p.hkv = a.hkv; p.group = a.hq / a.hkv; p.dim = a.dim;
   p.c = a.scale * kLog2e; p.scale = a.scale;
+  p.norms = d.norms;
   p.err = a.err;
   CUtensorMap m[4];
   if (int rc = attn_tmap(&m[0], a, a.q, a.hq, a.sq)) return rc;

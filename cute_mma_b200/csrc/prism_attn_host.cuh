@@ -23,6 +23,7 @@ struct AttnArgs {
   const void* d_o;            // backward: gradient of o with strides sdo
   AttnStrides sdo;
   float* delta;               // backward: scratch hq x rows
+  float* norms;               // backward in fp16: scratch of 2, or null
   void *dq, *dk, *dv;         // backward: rows x heads x dim, contiguous
   int* err;
   cudaStream_t stream;

@@ -73,14 +73,14 @@ extern "C" int prism_attn_fwd(const void* q, const void* k, const void* v, void*
   return launch_attn_fwd(a);
 }
 
-extern "C" int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
-                              const void* o_low, void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len,
-                              int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
-                              const long long* strides, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int prism_attn_bwd_scaled(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                                     const void* o_low, void* dq, void* dk, void* dv, float* delta, float* norms, const int* cu_seqlens,
+                                     int n_seqs, int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+                                     const long long* strides, void* workspace, size_t workspace_bytes, void* stream) {
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = const_cast<void*>(o); a.lse = const_cast<float*>(lse); a.d_o = d_o;
   a.low = const_cast<uint8_t*>(static_cast<const uint8_t*>(o_low));
-  a.dq = dq; a.dk = dk; a.dv = dv; a.delta = delta;
+  a.dq = dq; a.dk = dk; a.dv = dv; a.delta = delta; a.norms = norms;
   a.cu = cu_seqlens; a.n = n_seqs; a.len = seq_len; a.rows = rows;
   a.hq = heads; a.hkv = kv_heads; a.dim = head_dim; a.dtype = dtype; a.scale = scale;
   if (int rc = check_attn("prism_attn_bwd", a, strides, 12)) return rc;
@@ -92,6 +92,14 @@ extern "C" int prism_attn_bwd(const void* d_o, const void* q, const void* k, con
   a.err = static_cast<int*>(workspace);
   a.stream = static_cast<cudaStream_t>(stream);
   return launch_attn_bwd(a);
+}
+
+extern "C" int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                              const void* o_low, void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len,
+                              int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+                              const long long* strides, void* workspace, size_t workspace_bytes, void* stream) {
+  return prism_attn_bwd_scaled(d_o, q, k, v, o, lse, o_low, dq, dk, dv, delta, nullptr, cu_seqlens, n_seqs, seq_len, rows, heads, kv_heads,
+                               head_dim, dtype, scale, strides, workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t prism_attn_decode_scratch_bytes(int head_dim) {

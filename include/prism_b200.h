@@ -225,6 +225,13 @@ int prism_attn_bwd(const void* d_o, const void* q, const void* k, const void* v,
                    const void* o_low, void* dq, void* dk, void* dv, float* delta, const int* cu_seqlens, int n_seqs, int seq_len, int rows,
                    int heads, int kv_heads, int head_dim, int dtype, float scale, const long long* strides,
                    void* workspace, size_t workspace_bytes, void* stream);
+/* The same for fp16 gradients of any size: norms is scratch of 2 fp32 (any contents, not shared by calls that overlap), where
+ * the largest norms of d_o's and v's rows are taken first; dS, which is rounded to 16 bits between two products, then has a
+ * power of two that puts it into the type's range.  NULL, or bf16: prism_attn_bwd. */
+int prism_attn_bwd_scaled(const void* d_o, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                          const void* o_low, void* dq, void* dk, void* dv, float* delta, float* norms, const int* cu_seqlens,
+                          int n_seqs, int seq_len, int rows, int heads, int kv_heads, int head_dim, int dtype, float scale,
+                          const long long* strides, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Attention of one query row per sequence over its keys and values so far (serving: the next token).
  * q, o: n_seqs x heads x head_dim; k, v: n_seqs x room x kv_heads x head_dim, of which the first lengths[i] rows of sequence
