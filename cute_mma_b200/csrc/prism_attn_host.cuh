@@ -1,6 +1,8 @@
 // Host side of the attention kernels: their arguments, tensor maps and grids.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda_runtime.h>
 
 #include "prism_attn.cuh"
@@ -36,13 +38,13 @@ int launch_attn_decode(const AttnArgs& a, const int* lengths, float* scratch, in
 size_t attn_decode_scratch_bytes(int dim, int num_sms);
 
 // Tiles of bm rows over all sequences.  Packed: the lengths stand on the GPU; n sequences of `rows` rows have at most
-// (rows + n (bm - 1)) / bm tiles, and one more CTA row sees to the rows of no sequence.
+// (rows + n (bm - 1)) / bm tiles, nor more than they have rows, and one more CTA row sees to the rows of no sequence.
 inline int attn_rows(const AttnArgs& a, int bm, int heads, AttnRows* r) {
   r->cu = a.cu; r->n = a.n; r->len = a.len; r->rows = a.rows;
   long long tiles;
   if (a.rows == 0) tiles = 0;
   else if (a.cu == nullptr) tiles = (long long)a.n * ((a.len + bm - 1) / bm);
-  else tiles = ((long long)a.rows + (long long)a.n * (bm - 1)) / bm + 1;
+  else tiles = std::min(((long long)a.rows + (long long)a.n * (bm - 1)) / bm, (long long)a.rows) + 1;
   if (tiles * heads > 0x7fffffffll) return fail(PRISM_ERR_UNSUPPORTED, "attention: more than 2^31 tiles");
   r->tiles = (int)tiles;
   return PRISM_OK;
