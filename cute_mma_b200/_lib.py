@@ -18,7 +18,7 @@ SOURCES = ["prism_abi.cu", "prism_fwd.cu", "prism_fwd_small.cu", "prism_bwd_db.c
            "prism_bwd_dadr_f16.cu", "prism_bwd_dadr_bf16.cu", "prism_fwd_noalloc.cu", "prism_cayley.cu", "prism_peer_reduce.cu",
            "prism_shuffle.cu", "prism_decoder_abi.cu", "prism_attn_fwd.cu", "prism_attn_bwd.cu",
            "prism_attn_decode.cu", "prism_norm.cu"]
-HEADERS = ["prism_common.cuh", "prism_host.cuh", "prism_kernels.cuh", "prism_bwd_dadr_kernel.cuh", "prism_plan.h", "prism_attn.cuh",
+HEADERS = ["prism_common.cuh", "prism_host.cuh", "prism_kernels.cuh", "prism_bwd_dadr_kernel.cuh", "prism_plan.h", "prism_seen.h", "prism_attn.cuh",
            "prism_attn_host.cuh", "prism_norm.cuh"]
 PUBLIC_HEADER = os.path.join(os.path.dirname(_HERE), "include", "prism_b200.h")
 

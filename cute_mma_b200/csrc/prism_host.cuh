@@ -10,6 +10,7 @@
 #include <stdio.h>
 
 #include "prism_common.cuh"
+#include "prism_seen.h"
 
 namespace prism {
 
@@ -107,16 +108,13 @@ inline int make_tmap_2d(CUtensorMap* out, int dt, const void* base, uint64_t row
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize, set once per (kernel, device, size) instead of on every launch.
 inline int set_max_dynamic_smem(const void* kernel, int bytes, const char* what) {
-  struct Entry { const void* fn; int dev, bytes; };
-  static thread_local Entry seen[64];
-  static thread_local int n_seen = 0;
+  static thread_local SeenKernels seen;   // (zeros)
   int dev = 0;
   (void)cudaGetDevice(&dev);
-  for (int i = 0; i < n_seen; ++i)
-    if (seen[i].fn == kernel && seen[i].dev == dev && seen[i].bytes >= bytes) return PRISM_OK;
+  if (seen.has(kernel, dev, bytes)) return PRISM_OK;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(PRISM_ERR_CUDA, "%s: cannot set %d B of shared memory: %s", what, bytes, cudaGetErrorString(e));
-  if (n_seen < 64) seen[n_seen++] = Entry{kernel, dev, bytes};
+  seen.add(kernel, dev, bytes);
   return PRISM_OK;
 }
 
