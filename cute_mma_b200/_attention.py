@@ -92,6 +92,12 @@ def _tma_rows(t):
     return t, s
 
 
+def _whole(t):
+    """A saved tensor as it was saved: contiguous from a 16-byte boundary (saved-tensor hooks may have handed back another layout)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
 def _attn_forward(q, k, v, cu_seqlens, scale, train):
     """(o, lse, o_low), the latter two for the backward and None without it: the rows' log-sums, and what rounding o took
     (the backward needs do . o of every row more exactly than o as rounded gives it).  q, k, v as checked."""
@@ -130,8 +136,8 @@ def _attn_backward(d_o, q, k, v, o, lse, low, cu_seqlens, scale, need_dq=True, n
     dk, dv = (k.new_empty(k.shape) if need_dkv else None for _ in range(2))
     if rows == 0 or not (need_dq or need_dkv):
         return dq, dk, dv
-    # (saved-tensor hooks may have handed back another layout)
-    o, lse, low = o.contiguous(), lse.contiguous(), low.contiguous()
+    o, lse, low = _whole(o), _whole(lse), _whole(low)
+    cu_seqlens = None if cu_seqlens is None else _whole(cu_seqlens)
     d_o, sdo = _tma_rows(d_o)
     q, sq = _tma_rows(q)
     k, sk = _tma_rows(k)
