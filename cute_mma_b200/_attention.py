@@ -14,7 +14,7 @@ import torch
 
 from . import _functional as F
 from . import _lib
-from ._module import _plain_eager, _plain_grad
+from ._module import _plain_eager, _plain_grad, _refuse_tangents
 
 _MOST_ROWS = (1 << 31) - 257   # (the kernels' row numbers, rounded up to whole tiles, are 32-bit)
 _MOST_SEQUENCES = 1 << 20      # (packed)
@@ -237,6 +237,7 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             return _AttentionFn.apply(q, k, v, cu_seqlens, scale)
         return _attn_forward(q, k, v, cu_seqlens, scale, False)[0]
+    _refuse_tangents("causal_attention", q, k, v)
     return _attention_op(q, k, v, cu_seqlens, scale)[0]
 
 
@@ -311,4 +312,7 @@ def decode_attention(q, k, v, lengths, scale=None):
     """
     _check_decode(q, k, v, lengths)
     scale = _check_scale(scale, q.shape[-1])
-    return (_decode if _plain_eager(q, k, v, lengths) else _decode_op)(q, k, v, lengths, scale)
+    if _plain_eager(q, k, v, lengths):
+        return _decode(q, k, v, lengths, scale)
+    _refuse_tangents("decode_attention", q, k, v)
+    return _decode_op(q, k, v, lengths, scale)

@@ -242,6 +242,15 @@ def _plain_grad(dC) -> bool:
         return False
 
 
+def _refuse_tangents(what, *tensors) -> None:
+    """For operators without a forward-mode formula: a custom op drops tangents without a word, which reads as a derivative of zero.
+    (Called where ``_plain_eager`` is not true; no tangent gets that far.)"""
+    if torch.compiler.is_compiling():
+        return
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _layer_forward(A, weight, P, bias, ib, seeds, group_size, reconn_sz, activation, dropout_p, fold, cayley):
     """(C, and weight, R and internal bias as the backward needs them: the operands themselves, or what was made of
     them here).  P is R, or the Cayley parameter it is made from."""

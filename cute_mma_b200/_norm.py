@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from . import _functional as F
 from . import _lib
-from ._module import _plain_eager, _plain_grad
+from ._module import _plain_eager, _plain_grad, _refuse_tangents
 
 MAX_COLS = 16384
 
@@ -201,6 +201,7 @@ def layer_norm(x, weight, bias=None, eps: float = 1e-5, residual=None):
             return _NormFn.apply(x, weight, bias, eps, residual)
         y, s, _ = _norm_forward(x, weight, bias, eps, residual, False)
         return y if residual is None else (y, s)
+    _refuse_tangents("layer_norm", x, weight, bias, residual)
     y, s, _ = _norm_op(x, weight, bias, eps, residual)
     return y if residual is None else (y, s)
 

@@ -1,5 +1,5 @@
 """Norm and attention under what has to see their custom ops: compilation, dispatch modes, batches of output gradients, vmap,
-views with the negative bit, saved tensors of another layout."""
+forward-mode differentiation, views with the negative bit, saved tensors of another layout."""
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -123,6 +123,28 @@ def test_vmap():
     got = torch.func.vmap(cp.decode_attention)(qd, cache, cache, n)
     assert torch.equal(got, torch.stack([cp.decode_attention(a, b, b, c) for a, b, c in zip(qd, cache, n)]))
     cp.check_device_status()
+
+
+def _decode():
+    n = torch.tensor([70, 0, 13], device=DEV, dtype=torch.int32)
+    return (lambda q, k, v: cp.decode_attention(q, k, v, n)), [_randn(3, 4, 64), _randn(3, 70, 2, 64, seed=1), _randn(3, 70, 2, 64, seed=2)]
+
+
+@gpu
+@pytest.mark.parametrize("make", [*OPS, _decode])
+def test_tangents_are_refused_not_dropped(make):
+    """No forward-mode formula exists: an error, not a derivative of zero; inputs without tangents pass, also inside a level."""
+    f, leaves = make()
+    leaves = [t.detach() for t in leaves]
+    want = _outs(f(*leaves))
+    fw = torch.autograd.forward_ad
+    for i in range(len(leaves)):
+        with fw.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            f(*[fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(leaves)])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: f(*leaves[:i], t, *leaves[i + 1:]), (leaves[i],), (torch.ones_like(leaves[i]),))
+    with fw.dual_level():
+        assert all(torch.equal(a, b) for a, b in zip(_outs(f(*leaves)), want))
 
 
 @gpu
