@@ -186,7 +186,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-template <bool POLL>
+template <bool POLL, int LIMITS = 1>
 __device__ __forceinline__ bool warp_wait_t(uint64_t* bar, uint32_t parity) {
   if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
   const long long t0 = clock64();
@@ -194,7 +194,7 @@ __device__ __forceinline__ bool warp_wait_t(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
       if (__all_sync(0xffffffffu, POLL ? mbar_test(bar, parity) : mbar_try_wait(bar, parity))) return true;
-    if (__any_sync(0xffffffffu, clock64() - t0 > PRISM_WAIT_LIMIT_CYCLES)) return false;
+    if (__any_sync(0xffffffffu, clock64() - t0 > LIMITS * PRISM_WAIT_LIMIT_CYCLES)) return false;
   }
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return warp_wait_t<true>(bar, parity); }
@@ -209,7 +209,6 @@ struct AttnSched {
   alignas(16) uint64_t answer[2];
   AttnWork work[2];
   int head[2];
-  unsigned idle;   // tiles that there are none of, so far
 };
 __device__ __forceinline__ void attn_sched_init(AttnSched& s, uint32_t consumers) {
   for (int i = 0; i < 2; ++i) {
@@ -217,7 +216,6 @@ __device__ __forceinline__ void attn_sched_init(AttnSched& s, uint32_t consumers
     mbar_init(&s.empty[i], consumers);
   }
   mbar_init(&s.answer_full, 1);
-  s.idle = 0;
 }
 __device__ __forceinline__ void clc_try_cancel(uint64_t* answer, uint64_t* bar) {
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
@@ -259,7 +257,6 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
     const AttnWork w = attn_find(rows, order, idx / heads, bm, late);
     if (w.tile < 0) {
       zero(w, head);
-      if (lane == 0) *static_cast<volatile unsigned*>(&s.idle) = s.idle + 1;
     } else {
       ok = warp_wait(&s.empty[r.idx], r.phase ^ 1);
       if (ok && lane == 0) {
@@ -283,32 +280,20 @@ __device__ __forceinline__ bool attn_schedule(AttnSched& s, const AttnRows& rows
     fence_proxy_async_smem();   // the answer is read before the next one may overwrite it
     __syncwarp();
   }
-  if (!ok || !warp_wait(&s.empty[r.idx], r.phase ^ 1)) return false;
+  // (also where a wait has run out: there is no more work for the others either)
+  if (!warp_wait(&s.empty[r.idx], r.phase ^ 1)) return false;
   if (lane == 0) {
     s.work[r.idx].tile = -1;
     mbar_arrive(&s.full[r.idx]);
   }
-  return true;
+  return ok;
 }
-// Waits for a piece of work.  The limit counts from the last tile that there was none of: a CTA may go through a million of
-// those, a microsecond or two each, before it finds the next one that there is.
-__device__ __forceinline__ bool attn_wait_work(AttnSched& s, const Ring& r) {
-  if (__all_sync(0xffffffffu, mbar_test(&s.full[r.idx], r.phase))) return true;
-  long long t0 = clock64();
-  unsigned idle = *static_cast<volatile unsigned*>(&s.idle);
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (__all_sync(0xffffffffu, mbar_test(&s.full[r.idx], r.phase))) return true;
-    const unsigned now = *static_cast<volatile unsigned*>(&s.idle);
-    if (now != idle) t0 = clock64();
-    idle = now;
-    if (__any_sync(0xffffffffu, clock64() - t0 > PRISM_WAIT_LIMIT_CYCLES)) return false;
-  }
-}
-// The next piece of work for one of the other warps: false at the end (or if the wait ran out, with ok false).
+// The next piece of work for one of the other warps: false at the end (or if the wait ran out, with ok false).  The limit is 32
+// times that of other waits: a CTA may go through millions of tiles that there are none of before it finds the next one that
+// there is, 12 ns each over all CTAs, 26 s for the largest grid.  The warp that looks has its own, short waits, and says so when one
+// has run out.  (A wait that looks for progress instead cost dk and dv 1 to 6 % of their time.)
 __device__ __forceinline__ bool attn_next(AttnSched& s, Ring& r, AttnWork* w, int* head, bool* ok) {
-  if (!attn_wait_work(s, r)) { *ok = false; return false; }
+  if (!warp_wait_t<true, 32>(&s.full[r.idx], r.phase)) { *ok = false; return false; }
   // (through shuffles: the compiler then knows that all lanes have the same)
   const AttnWork& o = s.work[r.idx];
   w->tile = __shfl_sync(0xffffffffu, o.tile, 0);
