@@ -229,7 +229,9 @@ def causal_attention(q, k, v, cu_seqlens=None, scale=None):
     ``(batch, rows, heads, head_dim)``, a batch of them.  float16 or bfloat16; ``heads`` a multiple of ``kv_heads``
     (neighbouring query heads share a key head); ``head_dim`` a multiple of 8 up to 128; ``scale`` positive, by default
     ``head_dim ** -0.5``.  Column ranges of one QKV matrix are read in place.
-    Probabilities are rounded to the inputs' type before they meet ``v``, everything else is summed in fp32.
+    Rounded to the inputs' type on the way are the probabilities, before they meet ``v`` (and ``do``), and in the backward their
+    gradients, before they meet ``k`` and ``q``, in fp16 with factors that keep them in its range; all else is summed in fp32.
+    Infinities and NaN reach the rows that see them.  In the gradients they also reach rows of the same 128 rows of their sequence.
     """
     _check_prompt(q, k, v, cu_seqlens)
     scale = _check_scale(scale, q.shape[-1])

@@ -13,8 +13,10 @@
 //
 // Measured, bf16, one sequence of 8192 rows, 16 heads: of 128, dk and dv 460 us (tensor pipe 57 % busy: bound by the chain
 // S -> P -> dS -> dk of a tile, whose two accumulators leave no TMEM for a second tile), dq 280 us (86 %: bound by the
-// tensor pipe); of 64, 335 and 208 us (38 and 46 %: bound by the arithmetic between the products).  delta takes 20 us.
-// As one call it is 770 us, 890 TFLOP/s of the five products that the mathematics needs, and 565 us, 610 TFLOP/s.
+// tensor pipe); of 64, 335 and 208 us (38 and 46 %: bound by the arithmetic between the products).  delta takes 14 and
+// 7 us (fp16, with norms: 27 and 14 us; dk and dv 478 and 355 us).
+// Together 742 us, 926 TFLOP/s of the five products that the mathematics needs, and 553 us, 621 TFLOP/s; replayed without a pause,
+// under the power cap, 845 and 565 us.
 #include "prism_attn.cuh"
 #include "prism_attn_host.cuh"
 #include "prism_host.cuh"

@@ -4,7 +4,9 @@
 // Bound by HBM: every element is read once and kept in registers (16 to 32 a thread) between the two sums of a row.  The
 // squares are taken of deviations from the mean, not as a difference of means, which would lose rows far from zero.
 // Measured, bf16, 16384 rows of 4096 with a residual (cold L2): forward 82 us for 537 MB, 6.5 TB/s, as fast as a copy;
-// backward 83 us for 537 MB and the weight gradients' second launch.  Rows of 768: 20.5 and 27.6 us for 101 MB.
+// backward 83 us for 537 MB and the weight gradients' second launch.  Rows of 768: 20.5 and 27.6 us for 101 MB.  Without a
+// residual 4096 rows of 8192 take 35 and 64 us, of 12288 57 and 158 us, of 16384 64 and 178 us: above 8192 columns a thread of the
+// backward has 32 of them and its registers do not hold their weights and sums (512 to 904 bytes of it in local memory).
 //
 // The threads of a row are 8 to 512, the first that hold its columns; up to 32 they are part of a warp and reduce by
 // shuffles, several rows to a CTA.  Rows of full 16-byte pieces move in those, others in pairs or singly.
@@ -446,7 +448,10 @@ int launch_bwd_t(const NormArgs& a) {
   return check_launch("layer norm backward");
 }
 
-// The smallest of these (threads of a row) x (columns of a thread) that holds the row.
+// The smallest of these (threads of a row) x (columns of a thread) that holds the row.  They go up by powers of two, with one
+// step between 512 and 1024, where the library's own decoder is: 65536 rows of 768 with a residual take 68 us forward and 80 us
+// backward, with the next instance 74 and 92 us (16384 x 544: 20.5 and 28.7, else 22.5 and 32.8); odd widths, which move two
+// bytes at a time, lose forward (16384 x 767: 45, else 41 us) and gain backward (68, else 78 us).
 template <int DT, int VEC>
 int by_width_fwd(const NormArgs& a) {
   if (a.cols <= 16 * 16) return launch_fwd_t<DT, VEC, 16, 16>(a);
