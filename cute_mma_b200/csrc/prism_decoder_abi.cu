@@ -4,11 +4,18 @@
 #include "prism_host.cuh"
 #include "prism_norm.cuh"
 
+#include <initializer_list>
+
 using namespace prism;
 
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned_to(size_t size, std::initializer_list<const void*> ptrs) {   // to their own elements
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % size != 0) return false;
+  return true;
+}
 
 int check_workspace(const char* what, void* workspace, size_t bytes) {
   if (workspace == nullptr || bytes < PRISM_WORKSPACE_HEADER_BYTES)
@@ -53,6 +60,8 @@ int check_attn(const char* what, const AttnArgs& a, const long long* strides, in
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.o) || !aligned16(a.d_o) || !aligned16(a.dq) ||
       !aligned16(a.dk) || !aligned16(a.dv) || !aligned16(a.low))
     return fail(PRISM_ERR_BAD_ARG, "%s: tensors must be 16-byte aligned", what);
+  if (!aligned_to(4, {a.lse, a.delta, a.norms, a.cu}))
+    return fail(PRISM_ERR_BAD_ARG, "%s: lse, delta, norms and cu_seqlens must be 4-byte aligned", what);
   return PRISM_OK;
 }
 
@@ -127,6 +136,7 @@ extern "C" int prism_attn_decode(const void* q, const void* k, const void* v, vo
     return fail(PRISM_ERR_BAD_ARG, "%s: null tensor", what);
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(scratch))
     return fail(PRISM_ERR_BAD_ARG, "%s: tensors must be 16-byte aligned", what);
+  if (!aligned_to(4, {lengths})) return fail(PRISM_ERR_BAD_ARG, "%s: lengths must be 4-byte aligned", what);
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.n = n_seqs; a.len = room;
@@ -152,6 +162,9 @@ int check_norm(const char* what, const NormArgs& a, int w_dtype) {
     return fail(PRISM_ERR_BAD_ARG, "%s: the parameters must be fp32 or of the rows' type", what);
   if (!(a.eps >= 0.f)) return fail(PRISM_ERR_BAD_ARG, "%s: eps must not be negative", what);
   if (a.weight == nullptr || (a.rows > 0 && a.x == nullptr)) return fail(PRISM_ERR_BAD_ARG, "%s: null tensor", what);
+  if (!aligned_to(2, {a.x, a.residual, a.y, a.sum, a.dy, a.dsum, a.dx}) || !aligned_to(4, {a.mean, a.rstd}) ||
+      !aligned_to(a.w_f32 ? 4 : 2, {a.weight, a.bias, a.dw, a.db}))
+    return fail(PRISM_ERR_BAD_ARG, "%s: tensors must be aligned to their elements", what);
   if (a.ldx < 0 || a.ldr < 0 || a.lddy < 0 || a.ldds < 0) return fail(PRISM_ERR_BAD_ARG, "%s: negative row stride", what);
   return PRISM_OK;
 }
